@@ -345,6 +345,26 @@ int w4_rowscale_fp8(const void *y, int y_dtype, uint8_t *q, float *row_scale, in
                     void *stream);
 
 /* ===================================================================== */
+/* 8-bit integer (W8A8) linears and the MoE layer around them             */
+/* ===================================================================== */
+
+/* Function applied to the input of w4_quant_s8 before it is quantised. */
+enum w4_quant_fn {
+    W4_FN_NONE = 0,     /* y = x                                                   x [M, K]  */
+    W4_FN_SILU_MUL = 1, /* y = g / (1 + exp(-g)) * u, gate g = x[:, :K], u = x[:, K:]  x [M, 2K] */
+    W4_FN_RELU2 = 2     /* y = max(x, 0)^2                                         x [M, K]  */
+};
+
+/* Per-token symmetric s8 quantisation with the MLP's activation in the same pass:
+ *   y = fn(x);  s = max|y| / 127 (1 if 0);  q = clamp(rint(y / s), -127, 127)
+ * x f16 / bf16 / f32 (x_dtype) as listed at w4_quant_fn, q s8 [M, K], scale f32 [M].  y is held
+ * in f32 and never rounded to x_dtype.  A row in which y has a NaN or an infinity gets that
+ * as its scale and zero codes, so products with it are NaN.  The arithmetic is that of
+ * w4_rmsnorm_quant_s8 without the norm (kernels/epilogue_quant/rmsnorm_epilogue.cpp:56-70).
+ * K % 16 == 0, x and q 16-byte aligned, M >= 0. */
+int w4_quant_s8(const void *x, int x_dtype, int fn, int8_t *q, float *scale, int M, int K, void *stream);
+
+/* ===================================================================== */
 /* tensor parallelism                                                     */
 /* ===================================================================== */
 

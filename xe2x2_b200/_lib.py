@@ -18,6 +18,7 @@ W4_F16, W4_BF16, W4_F32, W4_E4M3, W4_S8, W4_E4M3_ATOMS = range(6)
 W4_NVFP4_KN, W4_NVFP4_NK = 0, 1
 W4_ACT_W4A16, W4_ACT_NVFP4 = 0, 1
 W4_TP_COLUMN, W4_TP_ROW = 0, 1
+W4_FN_NONE, W4_FN_SILU_MUL, W4_FN_RELU2 = range(3)
 W4_OVERLAP_OFF, W4_OVERLAP_DEPENDENT, W4_OVERLAP_STATIC_WEIGHTS = 0, 1, 2
 W4_TP_UNIQUE_ID_BYTES = 128
 W4_WORKSPACE_SYNC_BYTES = 16384  # zeroed sync area at the start of every workspace
@@ -69,6 +70,7 @@ _SIGS = {
     "w4_nvfp4_lut_gemm_s8a": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _P]),
     "w4_rmsnorm_quant_s8": (_I, [_P, _P, _P, _I, _I, _F, _P]),
     "w4_rowscale_fp8": (_I, [_P, _I, _P, _P, _I, _I, _P]),
+    "w4_quant_s8": (_I, [_P, _I, _I, _P, _P, _I, _I, _P]),
     "w4_tp_get_unique_id": (_I, [_P]),
     "w4_tp_comm_init": (_I, [ctypes.POINTER(_P), _I, _I, _P, _I]),
     "w4_tp_comm_destroy": (_I, [_P]),

@@ -619,4 +619,21 @@ int w4_rowscale_fp8(const void *y, int y_dtype, uint8_t *q, float *row_scale, in
     return w4::rowscale_fp8(y, y_dtype, q, row_scale, M, N, S(stream));
 }
 
+// ------------------------------------------------------------------ 8-bit integer linears, MoE
+static bool float_dtype(int dt) { return dt == W4_F16 || dt == W4_BF16 || dt == W4_F32; }
+
+int w4_quant_s8(const void *x, int x_dtype, int fn, int8_t *q, float *scale, int M, int K, void *stream) {
+    w4::set_error("");
+    W4_REQUIRE(float_dtype(x_dtype), W4_ERR_INVALID, "x_dtype must be f16, bf16 or f32");
+    W4_REQUIRE(fn == W4_FN_NONE || fn == W4_FN_SILU_MUL || fn == W4_FN_RELU2, W4_ERR_INVALID,
+               "fn %d is not one of W4_FN_*", fn);
+    W4_REQUIRE(M >= 0 && K > 0, W4_ERR_INVALID, "M=%d K=%d", M, K);
+    W4_REQUIRE(K % 16 == 0 && K <= (1 << 28), W4_ERR_UNSUPPORTED, "K=%d must be a multiple of 16, at most 2^28", K);
+    if (M == 0) return W4_OK;
+    W4_REQUIRE(x && q && scale, W4_ERR_INVALID, "null pointer argument");
+    W4_REQUIRE(aligned(x, 16) && aligned(q, 16) && aligned(scale, 4), W4_ERR_INVALID,
+               "x and q must be 16-byte aligned, scale 4-byte");
+    return w4::quant_s8(x, x_dtype, fn, q, scale, M, K, S(stream));
+}
+
 }  // extern "C"

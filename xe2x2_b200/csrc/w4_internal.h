@@ -160,4 +160,7 @@ int rowscale_fp8(const void *y, int y_dtype, uint8_t *q, float *row_scale, int M
 int rowscale_fp8_amax(const float *y, unsigned int *rowmax, unsigned int *rowcnt, uint8_t *q, float *row_scale,
                       int M, int N, cudaStream_t st);
 
+// s8_quant.cu: per-token s8 quantisation of fn(x) (W4_FN_*)
+int quant_s8(const void *x, int x_dtype, int fn, int8_t *q, float *scale, int M, int K, cudaStream_t st);
+
 }  // namespace w4

@@ -381,6 +381,63 @@ def rowscale_fp8(y):
     return q, s
 
 
+# ===================================================================== 8-bit integer linears
+_FN = {None: L.W4_FN_NONE, "none": L.W4_FN_NONE, "silu_mul": L.W4_FN_SILU_MUL, "relu2": L.W4_FN_RELU2}
+_FLOATS = {torch.float16: L.W4_F16, torch.bfloat16: L.W4_BF16, torch.float32: L.W4_F32}
+
+
+def _tensor(t, name, dtype, shape, dev, optional=False):
+    """Check one argument of the operators below: its dtype(s), shape, device, dense layout."""
+    if t is None and optional:
+        return None
+    if not torch.is_tensor(t):
+        raise ValueError(f"{name} must be a tensor")
+    _need_cuda(t)
+    ok = t.dtype in dtype if isinstance(dtype, (dict, tuple)) else t.dtype == dtype
+    if not ok:
+        want = ", ".join(str(d) for d in dtype) if isinstance(dtype, (dict, tuple)) else dtype
+        raise ValueError(f"{name} must be {want}, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    if t.device != dev:
+        raise ValueError(f"{name} is on {t.device}, the first tensor on {dev}")
+    return _contig(t, name)
+
+
+def _call_on(dev, name, *args):
+    """Call an entry point on dev's current stream with dev as the current device."""
+    if dev.index == torch.cuda.current_device():
+        L.call(name, *args, _stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            L.call(name, *args, _stream(dev))
+
+
+def quant_s8(x, act=None):
+    """Per-token s8 quantisation of act(x), the activation applied in the same pass.
+
+    ``act``: None, ``"silu_mul"`` (x [M, 2K] = gate | up, y = silu(gate) * up) or ``"relu2"``
+    (y = max(x, 0)^2).  x f16 / bf16 / f32, K a multiple of 16 -> (q s8 [M, K], scale f32 [M])
+    with y ~ q * scale, scale = max|y| / 127 (1 for a zero row).  A row with a NaN or an infinity
+    gets zero codes and that value as its scale.
+    """
+    if act not in _FN:
+        raise ValueError(f"act must be None, 'silu_mul' or 'relu2', got {act!r}")
+    if not torch.is_tensor(x) or x.dim() != 2:
+        raise ValueError("x must be a 2-D tensor")
+    dev = x.device
+    M, K = x.shape
+    _tensor(x, "x", _FLOATS, (M, K), dev)
+    if _FN[act] == L.W4_FN_SILU_MUL:
+        if K % 2:
+            raise ValueError("silu_mul needs x [M, 2K] (gate | up)")
+        K //= 2
+    q = torch.empty((M, K), dtype=torch.int8, device=dev)
+    s = torch.empty(M, dtype=torch.float32, device=dev)
+    _call_on(dev, "w4_quant_s8", _p(x), _FLOATS[x.dtype], _FN[act], _p(q), _p(s), M, K)
+    return q, s
+
+
 # ===================================================================== torch.ops.w4
 _registered = False
 
