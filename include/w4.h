@@ -364,6 +364,52 @@ enum w4_quant_fn {
  * K % 16 == 0, x and q 16-byte aligned, M >= 0. */
 int w4_quant_s8(const void *x, int x_dtype, int fn, int8_t *q, float *scale, int M, int K, void *stream);
 
+/* Scores of w4_moe_route, and how a group of experts is scored. */
+enum w4_moe_score {
+    W4_SCORE_SOFTMAX = 0,
+    W4_SCORE_SIGMOID = 1
+};
+enum w4_moe_group_score {
+    W4_GROUP_MAX = 0, /* the group's best expert */
+    W4_GROUP_TOP2 = 1 /* the sum of its two best */
+};
+
+/* MoE router: the top_k experts of every token with their weights, and the batch's order by expert.
+ *
+ * logits [T, E] f16 / bf16 / f32.  p = softmax(logits) or sigmoid(logits); the choice is by
+ * p + bias (bias f32 [E] or NULL), the weights are p without the bias.
+ *   - groups > 1: the experts form `groups` equal runs, each scored by W4_GROUP_MAX or
+ *     W4_GROUP_TOP2 of p + bias; only the topk_group best groups' experts can be chosen.
+ *   - ids i32 [T, top_k], best first; equal scores go to the lower index.  Scores are compared
+ *     in 64 bits (without a bias and group sums: as logits).
+ *   - weights f32 [T, top_k] = scaling * p, divided by their sum with renorm (0 if that is 0).
+ * An expert whose logit is -inf (or whose bias is -inf or NaN) is never chosen.  A token that has
+ * fewer than top_k experts to choose from gets id -1 and weight 0 in the slots left over, so a row
+ * of -inf (padding) goes nowhere.  A NaN logit counts as -inf for the choice, and every weight of
+ * its token is NaN.  An infinite logit counts as the largest finite one.
+ *
+ * The order by expert (all three or none):
+ *   offsets i32 [E + 1]:      expert e's rows are [offsets[e], offsets[e + 1]), ordered by token
+ *   rows    i32 [T * top_k]:  the token of each row, -1 behind offsets[E]
+ *   slots   i32 [T, top_k]:   the row of each (token, choice), -1 where id is -1
+ * The reference has the router as a kernel of its own (kernels/nemotron/moe_router.cpp).
+ * 1 <= E <= 512, top_k <= 32 and at most topk_group * E / groups, groups <= 32 and a divisor of E
+ * (W4_GROUP_TOP2 needs two experts a group); T >= 0.  workspace: plain scratch of
+ * w4_moe_route_workspace_bytes (no sync area; may be NULL where that is 0). */
+size_t w4_moe_route_workspace_bytes(int T, int E);
+int w4_moe_route(const void *logits, int logits_dtype, const float *bias, int T, int E, int top_k, int score,
+                 int groups, int topk_group, int group_score, int renorm, float scaling, int32_t *ids,
+                 float *weights, int32_t *offsets, int32_t *rows, int32_t *slots, void *workspace,
+                 size_t workspace_bytes, void *stream);
+
+/* Weighted sum of each token's expert outputs, in f32, in the order of the choices:
+ *   out[t] = add[t] + sum_j weights[t, j] * y[slots[t, j]]
+ * y [rows, H] of y_dtype, out and add (or NULL) [T, H] of out_dtype, each f16 / bf16 / f32.  A slot
+ * outside [0, rows) counts as a row of zeros.  out may be add; it must not overlap y.
+ * 1 <= top_k <= 32, T >= 0, any H. */
+int w4_moe_combine(const void *y, int y_dtype, int rows, const int32_t *slots, const float *weights,
+                   const void *add, void *out, int out_dtype, int T, int top_k, int H, void *stream);
+
 /* ===================================================================== */
 /* tensor parallelism                                                     */
 /* ===================================================================== */

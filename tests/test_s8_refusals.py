@@ -42,3 +42,69 @@ def test_quant_s8_wrapper_refusals():
         ops.quant_s8(x, "gelu")
     with pytest.raises(ValueError, match="2-D"):
         ops.quant_s8(torch.zeros(64))
+
+
+def _with(call, ok):
+    def rc(**kw):
+        args = list(ok)
+        for i, v in kw.items():
+            args[int(i[1:])] = v
+        return call(*args)
+    return rc
+
+
+def test_moe_route_refusals():
+    lib = L.lib()
+    #       logits dtype  bias  T   E  k  score  G  tg gs  ren scale  ids  w    off   rows  slots ws   bytes   stream
+    ok = [_f(), L.W4_BF16, None, 300, 64, 6, 0, 1, 1, 0, 1, 1.0, _f(), _f(), _f(), _f(), _f(), _f(), 1 << 20, None]
+    rc = _with(lib.w4_moe_route, ok)
+    for i in (0, 12, 13):
+        assert rc(**{f"_{i}": None}) == L.W4_ERR_INVALID
+    for i in (14, 15, 16):  # the plan's tensors come together
+        assert rc(**{f"_{i}": None}) == L.W4_ERR_INVALID and b"together" in lib.w4_last_error()
+    assert rc(_1=L.W4_E4M3) == L.W4_ERR_INVALID
+    assert rc(_3=-1) == L.W4_ERR_INVALID
+    assert rc(_4=0) == L.W4_ERR_INVALID
+    assert rc(_4=513) == L.W4_ERR_UNSUPPORTED
+    assert rc(_5=0) == L.W4_ERR_INVALID
+    assert rc(_5=33) == L.W4_ERR_UNSUPPORTED
+    assert rc(_4=4, _5=6) == L.W4_ERR_INVALID            # more than there are
+    assert rc(_6=2) == L.W4_ERR_INVALID and rc(_9=2) == L.W4_ERR_INVALID
+    assert rc(_7=5) == L.W4_ERR_INVALID                  # does not divide 64
+    assert rc(_7=8, _8=9) == L.W4_ERR_INVALID and rc(_7=8, _8=0) == L.W4_ERR_INVALID
+    assert rc(_7=16, _8=1, _5=6) == L.W4_ERR_INVALID     # 4 experts to choose 6 from
+    assert rc(_4=32, _7=32, _8=8, _9=1) == L.W4_ERR_INVALID  # top 2 of groups of one
+    assert rc(_7=64, _8=64) == L.W4_ERR_UNSUPPORTED
+    assert rc(_3=2**30) == L.W4_ERR_UNSUPPORTED          # T * top_k past 2^31
+    assert rc(_17=None) == L.W4_ERR_INVALID and b"workspace" in lib.w4_last_error()
+    assert rc(_18=16) == L.W4_ERR_INVALID
+    assert rc(_0=_f(0x10001)) == L.W4_ERR_INVALID
+    assert lib.w4_moe_route_workspace_bytes(8, 64) == 0 and lib.w4_moe_route_workspace_bytes(0, 64) == 0
+    assert lib.w4_moe_route_workspace_bytes(8192, 256) >= 8192 // 1024 * 256 * 4
+
+
+def test_moe_combine_refusals():
+    lib = L.lib()
+    ok = [_f(), L.W4_BF16, 48, _f(), _f(), None, _f(0x90000), L.W4_BF16, 8, 6, 64, None]
+    rc = _with(lib.w4_moe_combine, ok)
+    for i in (0, 3, 4, 6):
+        assert rc(**{f"_{i}": None}) == L.W4_ERR_INVALID
+    assert rc(_1=L.W4_S8) == L.W4_ERR_INVALID and rc(_7=L.W4_E4M3) == L.W4_ERR_INVALID
+    assert rc(_2=-1) == L.W4_ERR_INVALID and rc(_8=-1) == L.W4_ERR_INVALID and rc(_10=0) == L.W4_ERR_INVALID
+    assert rc(_9=0) == L.W4_ERR_INVALID and rc(_9=33) == L.W4_ERR_UNSUPPORTED
+    assert rc(_6=_f()) == L.W4_ERR_INVALID               # out is y
+    assert rc(_8=0) == L.W4_OK
+
+
+def test_moe_wrapper_refusals():
+    x = torch.zeros(4, 8)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.moe_route(x, 2)
+    with pytest.raises(ValueError, match="score"):
+        ops.moe_route(x, 2, score="tanh")
+    with pytest.raises(ValueError, match="group_score"):
+        ops.moe_route(x, 2, group_score="sum")
+    with pytest.raises(ValueError, match="2-D"):
+        ops.moe_route(x[0], 2)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.moe_combine(x, torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, 2))

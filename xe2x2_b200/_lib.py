@@ -18,6 +18,8 @@ W4_F16, W4_BF16, W4_F32, W4_E4M3, W4_S8, W4_E4M3_ATOMS = range(6)
 W4_NVFP4_KN, W4_NVFP4_NK = 0, 1
 W4_ACT_W4A16, W4_ACT_NVFP4 = 0, 1
 W4_TP_COLUMN, W4_TP_ROW = 0, 1
+W4_SCORE_SOFTMAX, W4_SCORE_SIGMOID = 0, 1
+W4_GROUP_MAX, W4_GROUP_TOP2 = 0, 1
 W4_FN_NONE, W4_FN_SILU_MUL, W4_FN_RELU2 = range(3)
 W4_OVERLAP_OFF, W4_OVERLAP_DEPENDENT, W4_OVERLAP_STATIC_WEIGHTS = 0, 1, 2
 W4_TP_UNIQUE_ID_BYTES = 128
@@ -71,6 +73,9 @@ _SIGS = {
     "w4_rmsnorm_quant_s8": (_I, [_P, _P, _P, _I, _I, _F, _P]),
     "w4_rowscale_fp8": (_I, [_P, _I, _P, _P, _I, _I, _P]),
     "w4_quant_s8": (_I, [_P, _I, _I, _P, _P, _I, _I, _P]),
+    "w4_moe_route_workspace_bytes": (_Z, [_I, _I]),
+    "w4_moe_route": (_I, [_P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _P, _P, _P, _P, _P, _P, _Z, _P]),
+    "w4_moe_combine": (_I, [_P, _I, _I, _P, _P, _P, _P, _I, _I, _I, _I, _P]),
     "w4_tp_get_unique_id": (_I, [_P]),
     "w4_tp_comm_init": (_I, [ctypes.POINTER(_P), _I, _I, _P, _I]),
     "w4_tp_comm_destroy": (_I, [_P]),

@@ -636,4 +636,64 @@ int w4_quant_s8(const void *x, int x_dtype, int fn, int8_t *q, float *scale, int
     return w4::quant_s8(x, x_dtype, fn, q, scale, M, K, S(stream));
 }
 
+size_t w4_moe_route_workspace_bytes(int T, int E) {
+    if (T <= 0 || E < 1 || E > w4::kMaxMoeExperts) return 0;
+    return w4::moe_route_workspace(T, E);
+}
+
+int w4_moe_route(const void *logits, int logits_dtype, const float *bias, int T, int E, int top_k, int score,
+                 int groups, int topk_group, int group_score, int renorm, float scaling, int32_t *ids,
+                 float *weights, int32_t *offsets, int32_t *rows, int32_t *slots, void *workspace,
+                 size_t workspace_bytes, void *stream) {
+    w4::set_error("");
+    W4_REQUIRE(float_dtype(logits_dtype), W4_ERR_INVALID, "logits_dtype must be f16, bf16 or f32");
+    W4_REQUIRE(score == W4_SCORE_SOFTMAX || score == W4_SCORE_SIGMOID, W4_ERR_INVALID,
+               "score %d is not one of W4_SCORE_*", score);
+    W4_REQUIRE(group_score == W4_GROUP_MAX || group_score == W4_GROUP_TOP2, W4_ERR_INVALID,
+               "group_score %d is not one of W4_GROUP_*", group_score);
+    W4_REQUIRE(T >= 0 && E >= 1 && top_k >= 1 && groups >= 1, W4_ERR_INVALID, "T=%d E=%d top_k=%d groups=%d", T, E,
+               top_k, groups);
+    W4_REQUIRE(E <= w4::kMaxMoeExperts && top_k <= w4::kMaxTopK && groups <= w4::kMaxGroups, W4_ERR_UNSUPPORTED,
+               "at most %d experts, top %d and %d groups (E=%d top_k=%d groups=%d)", w4::kMaxMoeExperts, w4::kMaxTopK,
+               w4::kMaxGroups, E, top_k, groups);
+    W4_REQUIRE(E % groups == 0 && topk_group >= 1 && topk_group <= groups, W4_ERR_INVALID,
+               "groups=%d must divide E=%d and topk_group=%d lie in 1..groups", groups, E, topk_group);
+    W4_REQUIRE(groups == 1 || group_score == W4_GROUP_MAX || E / groups >= 2, W4_ERR_INVALID,
+               "W4_GROUP_TOP2 needs at least two experts a group");
+    W4_REQUIRE(top_k <= topk_group * (E / groups), W4_ERR_INVALID, "top_k=%d experts out of %d that can be chosen",
+               top_k, topk_group * (E / groups));
+    W4_REQUIRE((long long)T * top_k <= 0x7FFFFFFFLL, W4_ERR_UNSUPPORTED, "T * top_k exceeds 2^31 - 1");
+    const bool plan = offsets || rows || slots;
+    if (T == 0 && !offsets) return W4_OK;
+    W4_REQUIRE(T == 0 || (logits && ids && weights), W4_ERR_INVALID, "logits, ids and weights are required");
+    W4_REQUIRE(!plan || (offsets && (T == 0 || (rows && slots))), W4_ERR_INVALID,
+               "offsets, rows and slots come together");
+    const size_t es = logits_dtype == W4_F32 ? 4 : 2;
+    W4_REQUIRE(aligned(logits, es) && aligned(bias, 4) && aligned(ids, 4) && aligned(weights, 4) &&
+                   aligned(offsets, 4) && aligned(rows, 4) && aligned(slots, 4),
+               W4_ERR_INVALID, "tensors must be aligned to their element size");
+    const size_t need = plan ? w4_moe_route_workspace_bytes(T, E) : 0;
+    W4_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 16)), W4_ERR_INVALID,
+               "a 16-byte aligned workspace of %zu bytes is needed (%zu given)", need, workspace_bytes);
+    return w4::moe_route(logits, logits_dtype, bias, T, E, top_k, score, groups, topk_group, group_score, renorm,
+                         scaling, ids, weights, offsets, rows, slots, workspace, S(stream));
+}
+
+int w4_moe_combine(const void *y, int y_dtype, int rows, const int32_t *slots, const float *weights,
+                   const void *add, void *out, int out_dtype, int T, int top_k, int H, void *stream) {
+    w4::set_error("");
+    W4_REQUIRE(float_dtype(y_dtype) && float_dtype(out_dtype), W4_ERR_INVALID,
+               "y_dtype and out_dtype must be f16, bf16 or f32");
+    W4_REQUIRE(T >= 0 && rows >= 0 && H >= 1 && top_k >= 1, W4_ERR_INVALID, "T=%d rows=%d H=%d top_k=%d", T, rows, H,
+               top_k);
+    W4_REQUIRE(top_k <= w4::kMaxTopK, W4_ERR_UNSUPPORTED, "top_k=%d exceeds %d", top_k, w4::kMaxTopK);
+    if (T == 0) return W4_OK;
+    W4_REQUIRE((y || rows == 0) && slots && weights && out, W4_ERR_INVALID, "null pointer argument");
+    W4_REQUIRE(out != y, W4_ERR_INVALID, "out must not be y");
+    W4_REQUIRE(aligned(y, y_dtype == W4_F32 ? 4 : 2) && aligned(out, out_dtype == W4_F32 ? 4 : 2) &&
+                   aligned(add, out_dtype == W4_F32 ? 4 : 2) && aligned(slots, 4) && aligned(weights, 4),
+               W4_ERR_INVALID, "tensors must be aligned to their element size");
+    return w4::moe_combine(y, y_dtype, rows, slots, weights, add, out, out_dtype, T, top_k, H, S(stream));
+}
+
 }  // extern "C"

@@ -163,4 +163,13 @@ int rowscale_fp8_amax(const float *y, unsigned int *rowmax, unsigned int *rowcnt
 // s8_quant.cu: per-token s8 quantisation of fn(x) (W4_FN_*)
 int quant_s8(const void *x, int x_dtype, int fn, int8_t *q, float *scale, int M, int K, cudaStream_t st);
 
+// moe.cu: the router with the batch's order by expert, and the weighted sum of expert outputs
+constexpr int kMaxTopK = 32, kMaxGroups = 32, kMaxMoeExperts = 512;
+size_t moe_route_workspace(int T, int E);
+int moe_route(const void *logits, int dtype, const float *bias, int T, int E, int k, int score, int groups,
+              int topk_group, int group_score, int renorm, float scaling, int *ids, float *weights, int *offsets,
+              int *rows, int *slots, void *workspace, cudaStream_t st);
+int moe_combine(const void *y, int y_dtype, int rows, const int *slots, const float *weights, const void *add,
+                void *out, int out_dtype, int T, int k, int H, cudaStream_t st);
+
 }  // namespace w4

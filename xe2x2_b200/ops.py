@@ -25,6 +25,7 @@ from __future__ import annotations
 import ctypes
 import threading
 import weakref
+from typing import NamedTuple
 
 import torch
 
@@ -436,6 +437,83 @@ def quant_s8(x, act=None):
     s = torch.empty(M, dtype=torch.float32, device=dev)
     _call_on(dev, "w4_quant_s8", _p(x), _FLOATS[x.dtype], _FN[act], _p(q), _p(s), M, K)
     return q, s
+
+
+# ===================================================================== MoE: router, combine
+class MoERouting(NamedTuple):
+    """What :func:`moe_route` returns.  ``ids`` i32 [T, k] (best first, -1: none), ``weights`` f32
+    [T, k], and the batch's order by expert: ``offsets`` i32 [E + 1] (expert e's rows are
+    [offsets[e], offsets[e + 1])), ``rows`` i32 [T * k] (each row's token, -1 behind
+    offsets[E]), ``slots`` i32 [T, k] (each choice's row, -1: none).  ``offsets.tolist()`` is what the
+    4-bit grouped GEMMs take."""
+    ids: torch.Tensor
+    weights: torch.Tensor
+    offsets: torch.Tensor
+    rows: torch.Tensor
+    slots: torch.Tensor
+
+
+_SCORES = {"softmax": L.W4_SCORE_SOFTMAX, "sigmoid": L.W4_SCORE_SIGMOID}
+_GROUP_SCORES = {"max": L.W4_GROUP_MAX, "top2": L.W4_GROUP_TOP2}
+
+
+def moe_route(logits, top_k, bias=None, score="softmax", renormalize=True, scaling=1.0, n_group=1, topk_group=1,
+              group_score="max") -> MoERouting:
+    """MoE router: logits [T, E] (f16 / bf16 / f32, E <= 512) -> :class:`MoERouting`.
+
+    Each token takes the ``top_k`` experts with the largest score + ``bias`` (f32 [E]), out of the
+    ``topk_group`` best of ``n_group`` equal groups when ``n_group`` > 1 (a group scored by its best
+    expert, ``group_score="max"``, or its two best, ``"top2"``); equal scores go to the lower index.
+    The weights are ``scaling`` * softmax / sigmoid scores without the bias, divided by their sum
+    with ``renormalize``.  A logit of -inf switches an expert off, a row of -inf (padding) goes
+    nowhere; a NaN logit makes its token's weights NaN.
+    """
+    if score not in _SCORES:
+        raise ValueError(f"score must be 'softmax' or 'sigmoid', got {score!r}")
+    if group_score not in _GROUP_SCORES:
+        raise ValueError(f"group_score must be 'max' or 'top2', got {group_score!r}")
+    if not torch.is_tensor(logits) or logits.dim() != 2:
+        raise ValueError("logits must be a 2-D tensor [tokens, experts]")
+    dev = logits.device
+    T, E = logits.shape
+    _tensor(logits, "logits", _FLOATS, (T, E), dev)
+    _tensor(bias, "bias", torch.float32, (E,), dev, optional=True)
+    top_k = int(top_k)
+    if top_k < 1:
+        raise ValueError(f"top_k must be at least 1, got {top_k}")
+    ids = torch.empty((T, top_k), dtype=torch.int32, device=dev)
+    weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
+    offsets = torch.empty(E + 1, dtype=torch.int32, device=dev)
+    rows = torch.empty(T * top_k, dtype=torch.int32, device=dev)
+    slots = torch.empty((T, top_k), dtype=torch.int32, device=dev)
+    need = L.lib().w4_moe_route_workspace_bytes(T, E)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _call_on(dev, "w4_moe_route", _p(logits), _FLOATS[logits.dtype], _p(bias), T, E, top_k, _SCORES[score],
+             int(n_group), int(topk_group), _GROUP_SCORES[group_score], int(bool(renormalize)), float(scaling), _p(ids),
+             _p(weights), _p(offsets), _p(rows), _p(slots), _p(ws), need)
+    return MoERouting(ids, weights, offsets, rows, slots)
+
+
+def moe_combine(y, slots, weights, add=None, out_dtype=None):
+    """Weighted sum of each token's expert outputs: out[t] = add[t] + sum_j weights[t, j] *
+    y[slots[t, j]] in f32 (a slot of -1 counts as zeros).  y [rows, H] f16 / bf16 / f32, slots i32 and
+    weights f32 [T, k] from :func:`moe_route`, ``add`` [T, H] of the output's dtype (a shared expert's
+    output, the residual stream) -> [T, H] of ``out_dtype`` (default: y's)."""
+    if not torch.is_tensor(y) or y.dim() != 2 or not torch.is_tensor(slots) or slots.dim() != 2:
+        raise ValueError("y must be [rows, H] and slots [tokens, top_k]")
+    dev = y.device
+    (rows, H), (T, k) = y.shape, slots.shape
+    out_dtype = out_dtype or y.dtype
+    _tensor(y, "y", _FLOATS, (rows, H), dev)
+    _tensor(slots, "slots", torch.int32, (T, k), dev)
+    _tensor(weights, "weights", torch.float32, (T, k), dev)
+    if out_dtype not in _FLOATS:
+        raise ValueError(f"out_dtype must be f16, bf16 or f32, got {out_dtype}")
+    _tensor(add, "add", out_dtype, (T, H), dev, optional=True)
+    out = torch.empty((T, H), dtype=out_dtype, device=dev)
+    _call_on(dev, "w4_moe_combine", _p(y), _FLOATS[y.dtype], rows, _p(slots), _p(weights), _p(add), _p(out),
+             _FLOATS[out_dtype], T, k, H)
+    return out
 
 
 # ===================================================================== torch.ops.w4
