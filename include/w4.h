@@ -364,6 +364,36 @@ enum w4_quant_fn {
  * K % 16 == 0, x and q 16-byte aligned, M >= 0. */
 int w4_quant_s8(const void *x, int x_dtype, int fn, int8_t *q, float *scale, int M, int K, void *stream);
 
+/* W8A8 GEMM:  C[m,n] = (sum_k a[m,k] * w[n,k]) * a_scale[m] * w_scale[n] + bias[n]
+ * a s8 [M, K] and a_scale f32 [M] as w4_quant_s8 or w4_rmsnorm_quant_s8 write them; w s8 [N, K]
+ * (K contiguous), w_scale f32 [N]; bias f32 [N] or NULL.  The integer sum is exact, what follows is
+ * f32.  c [M, N] of c_dtype W4_F16 / W4_BF16 / W4_F32, or W4_E4M3 with row_scale f32 [M] as in
+ * w4_gptq_gemm.  K % 16 == 0, K <= 131056 (the sum fits 32 bits), any N >= 1, M >= 0; a and w
+ * 16-byte aligned.  workspace: plain scratch (no sync area), needed for W4_E4M3 only (may be NULL
+ * where w4_s8_gemm_workspace_bytes is 0).
+ * The reference's s8 x s8 tiles with a scale per row and column: kernels/esimd_dpas/dpas_s8_sc.cpp:122-208. */
+size_t w4_s8_gemm_workspace_bytes(int M, int N, int K, int c_dtype);
+int w4_s8_gemm(const int8_t *a, const float *a_scale, const int8_t *w, const float *w_scale, const float *bias,
+               void *c, int c_dtype, float *row_scale, int M, int N, int K, void *workspace,
+               size_t workspace_bytes, void *stream);
+
+/* Grouped (MoE) W8A8 GEMM: expert e multiplies rows [offsets[e], offsets[e+1]) of the batch by its
+ * slice of w s8 [E, N, K] with w_scale f32 [E, N] and bias f32 [E, N] or NULL; c [R, N].
+ * offsets: i32 [E + 1] in DEVICE memory, nondecreasing from 0 to at most R, as w4_moe_route writes
+ * them (never read by the host; values outside [0, R] or out of order are clamped, so no row
+ * outside the buffers is touched).  Rows of c (and of row_scale) behind offsets[E] are left as
+ * they are.
+ * rows == NULL: row r of the batch is row r of a s8 [R, K], a_rows = R.  Else row r is row rows[r] of
+ * a s8 [a_rows, K] (i32 [R] in device memory, as w4_moe_route writes it), with its a_scale; an index
+ * outside [0, a_rows) counts as a row of zeros.
+ * 1 <= E <= 512; types, K, alignment and workspace as w4_s8_gemm, with R for M.
+ * The reference chains its s8 expert GEMMs on one queue: kernels/esimd_dpas/moe_group_s8_m1.cpp:1-7. */
+size_t w4_s8_gemm_grouped_workspace_bytes(int R, int N, int K, int c_dtype);
+int w4_s8_gemm_grouped(const int8_t *a, const float *a_scale, int a_rows, const int8_t *w, const float *w_scale,
+                       const float *bias, const int32_t *offsets, const int32_t *rows, int E, void *c, int c_dtype,
+                       float *row_scale, int R, int N, int K, void *workspace, size_t workspace_bytes,
+                       void *stream);
+
 /* Scores of w4_moe_route, and how a group of experts is scored. */
 enum w4_moe_score {
     W4_SCORE_SOFTMAX = 0,

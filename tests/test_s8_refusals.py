@@ -108,3 +108,49 @@ def test_moe_wrapper_refusals():
         ops.moe_route(x[0], 2)
     with pytest.raises(ValueError, match="CUDA"):
         ops.moe_combine(x, torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, 2))
+
+
+def test_s8_gemm_refusals():
+    lib = L.lib()
+    #       a     as    w     ws    bias  c     dtype      rs    M  N   K   ws    bytes stream
+    ok = [_f(), _f(), _f(), _f(), None, _f(), L.W4_BF16, None, 4, 64, 64, None, 0, None]
+    rc = _with(lib.w4_s8_gemm, ok)
+    for i in (0, 1, 2, 3, 5):
+        assert rc(**{f"_{i}": None}) == L.W4_ERR_INVALID
+    for i in (0, 2):
+        assert rc(**{f"_{i}": _f(0x10008)}) == L.W4_ERR_INVALID and b"aligned" in lib.w4_last_error()
+    assert rc(_6=L.W4_S8) == L.W4_ERR_INVALID
+    assert rc(_8=-1) == L.W4_ERR_INVALID and rc(_9=0) == L.W4_ERR_INVALID and rc(_10=0) == L.W4_ERR_INVALID
+    assert rc(_10=72) == L.W4_ERR_UNSUPPORTED and rc(_10=131072) == L.W4_ERR_UNSUPPORTED
+    assert rc(_6=L.W4_E4M3) == L.W4_ERR_INVALID and b"row_scale" in lib.w4_last_error()
+    assert rc(_6=L.W4_E4M3, _7=_f()) == L.W4_ERR_INVALID and b"workspace" in lib.w4_last_error()
+    assert rc(_8=0, _0=None) == L.W4_OK
+    assert lib.w4_s8_gemm_workspace_bytes(4, 64, 64, L.W4_BF16) == 0
+    assert lib.w4_s8_gemm_workspace_bytes(4, 64, 64, L.W4_E4M3) == 1024
+
+
+def test_s8_gemm_grouped_refusals():
+    lib = L.lib()
+    #       a     as  a_rows w    ws    bias  off   rows E  c     dtype      rs   R  N   K   ws    bytes stream
+    ok = [_f(), _f(), 8, _f(), _f(), None, _f(), None, 4, _f(), L.W4_BF16, None, 8, 64, 64, None, 0, None]
+    rc = _with(lib.w4_s8_gemm_grouped, ok)
+    for i in (0, 1, 3, 4, 6, 9):
+        assert rc(**{f"_{i}": None}) == L.W4_ERR_INVALID
+    assert rc(_2=7) == L.W4_ERR_INVALID and b"a_rows" in lib.w4_last_error()
+    assert rc(_2=0, _7=_f()) == L.W4_ERR_INVALID
+    assert rc(_8=0) == L.W4_ERR_INVALID and rc(_8=513) == L.W4_ERR_UNSUPPORTED
+    assert rc(_12=-1) == L.W4_ERR_INVALID and rc(_14=24) == L.W4_ERR_UNSUPPORTED
+    assert rc(_10=L.W4_E4M3) == L.W4_ERR_INVALID
+    assert rc(_0=_f(0x10004)) == L.W4_ERR_INVALID and rc(_6=_f(0x10002)) == L.W4_ERR_INVALID
+    assert rc(_12=0, _2=0) == L.W4_OK
+
+
+def test_s8_wrapper_refusals():
+    a, s = torch.zeros(4, 64, dtype=torch.int8), torch.zeros(4)
+    w, ws = torch.zeros(8, 64, dtype=torch.int8), torch.zeros(8)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.s8_gemm(a, s, w, ws)
+    with pytest.raises(ValueError):
+        ops.s8_gemm(a, s, w[0], ws)
+    with pytest.raises(ValueError):
+        ops.s8_gemm_grouped(a, s, w, ws, torch.zeros(2, dtype=torch.int32))

@@ -73,6 +73,10 @@ _SIGS = {
     "w4_rmsnorm_quant_s8": (_I, [_P, _P, _P, _I, _I, _F, _P]),
     "w4_rowscale_fp8": (_I, [_P, _I, _P, _P, _I, _I, _P]),
     "w4_quant_s8": (_I, [_P, _I, _I, _P, _P, _I, _I, _P]),
+    "w4_s8_gemm_workspace_bytes": (_Z, [_I, _I, _I, _I]),
+    "w4_s8_gemm": (_I, [_P, _P, _P, _P, _P, _P, _I, _P, _I, _I, _I, _P, _Z, _P]),
+    "w4_s8_gemm_grouped_workspace_bytes": (_Z, [_I, _I, _I, _I]),
+    "w4_s8_gemm_grouped": (_I, [_P, _P, _I, _P, _P, _P, _P, _P, _I, _P, _I, _P, _I, _I, _I, _P, _Z, _P]),
     "w4_moe_route_workspace_bytes": (_Z, [_I, _I]),
     "w4_moe_route": (_I, [_P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _P, _P, _P, _P, _P, _P, _Z, _P]),
     "w4_moe_combine": (_I, [_P, _I, _I, _P, _P, _P, _P, _I, _I, _I, _I, _P]),

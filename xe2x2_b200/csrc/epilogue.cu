@@ -90,9 +90,10 @@ __device__ __forceinline__ float load_as_f(const void *p, size_t i) {
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads)
 rowscale_fp8_kernel(const void *__restrict__ y, uint8_t *__restrict__ q,
-                    float *__restrict__ row_scale, int N) {
+                    float *__restrict__ row_scale, int N, const int *__restrict__ limit) {
     __shared__ float sh[32];
     const int row = blockIdx.x;
+    if (limit && row >= *limit) return;
     const size_t base = (size_t)row * N;
     float amax = 0.f;
     for (int j = threadIdx.x; j < N; j += blockDim.x) amax = fmaxf(amax, fabsf(load_as_f<T>(y, base + j)));
@@ -147,10 +148,11 @@ int rowscale_fp8_amax(const float *y, unsigned int *rowmax, unsigned int *rowcnt
 }
 
 int rowscale_fp8(const void *y, int y_dtype, uint8_t *q, float *row_scale, int M, int N,
-                 cudaStream_t st) {
-    if (y_dtype == W4_F32) rowscale_fp8_kernel<float><<<M, kRowThreads, 0, st>>>(y, q, row_scale, N);
-    else if (y_dtype == W4_BF16) rowscale_fp8_kernel<__nv_bfloat16><<<M, kRowThreads, 0, st>>>(y, q, row_scale, N);
-    else rowscale_fp8_kernel<__half><<<M, kRowThreads, 0, st>>>(y, q, row_scale, N);
+                 cudaStream_t st, const int *limit) {
+    if (y_dtype == W4_F32) rowscale_fp8_kernel<float><<<M, kRowThreads, 0, st>>>(y, q, row_scale, N, limit);
+    else if (y_dtype == W4_BF16)
+        rowscale_fp8_kernel<__nv_bfloat16><<<M, kRowThreads, 0, st>>>(y, q, row_scale, N, limit);
+    else rowscale_fp8_kernel<__half><<<M, kRowThreads, 0, st>>>(y, q, row_scale, N, limit);
     W4_LAUNCH_CHECK();
     return W4_OK;
 }

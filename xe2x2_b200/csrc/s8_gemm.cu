@@ -1,0 +1,494 @@
+// s8_gemm.cu -- W8A8 GEMM on the 5th-generation tensor cores (tcgen05.mma kind::i8, sm_100a), for
+// one matrix and for a batch sorted by expert.
+//
+// Contract: w4_s8_gemm / w4_s8_gemm_grouped,
+//   C[m, n] = f(sum_k A[m, k] * W[n, k]) * a_scale[m] * w_scale[n] + bias[n]
+// with the integer sum exact (s32 in TMEM; |sum| <= 2^14 K < 2^31) and every step behind it in f32.
+//
+// The weights are the MMA's M side (128 output channels a tile) and the tokens its N side, so that
+// one kernel serves every batch: N is 16 for a decode step and 256 for a prompt, and the MMA's N
+// follows the rows that a tile has.  Both operands are K-major 128-byte lines, 128-byte swizzle,
+// fetched by TMA; K is padded with zeros by the copy itself.  Token rows may be gathered through an
+// index (tile::gather4, four rows a copy).  Warp 0 produces, warp 1 issues the MMAs, warps 2-5 read
+// the sums out of TMEM (two accumulators: one fills while the other is read), scale and store.
+// Every wait is bounded; no copy names more than one CTA.
+#include <mutex>
+
+#include "tma_util.cuh"
+#include "w4_common.cuh"
+#include "w4_internal.h"
+
+namespace w4 {
+
+static __device__ unsigned int g_s8_timeout;  // a bounded wait expired (sticky until read)
+
+namespace s8g {
+
+constexpr int BN = 128, BK = 128;  // output channels and bytes of K in a stage
+constexpr int kThreads = 6 * 32, kEpi = 4;
+constexpr uint32_t W_BYTES = BN * BK;
+
+enum Mode { kDense = 0, kGrouped = 1, kGathered = 2 };
+
+struct Args {
+    const float *a_scale, *w_scale, *bias;
+    const int *offsets, *src;
+    void *c;
+    int c_dtype, M, a_rows, N, K, E;
+    int bt, box;  // token rows of a tile (a multiple of 16), of one token copy
+    int ntn;      // column tiles
+};
+
+// BT token rows at most, S stages, two accumulators of BT columns.
+template <int BT> struct Cfg {
+    static constexpr uint32_t T_BYTES = BT * BK, STAGE = W_BYTES + T_BYTES;
+    static constexpr int S = BT == 256 ? 4 : BT == 128 ? 6 : BT == 64 ? 9 : 12;
+    static constexpr uint32_t TMEM_COLS = 2 * BT < 32 ? 32 : 2 * BT;
+    static constexpr uint32_t BAR_OFF = S * STAGE, AS_OFF = BAR_OFF + (2 * S + 5) * 8 / 16 * 16 + 16,
+                              MISC_OFF = AS_OFF + 2 * BT * 4, TILE_OFF = MISC_OFF + 16;
+    static constexpr uint32_t LD = BT < 32 ? BT : 32;  // columns of one TMEM read
+    static constexpr size_t smem(int E) { return TILE_OFF + (size_t)2 * (E + 1) * 4 + 1024; }
+    static_assert(TILE_OFF + 2 * (kMaxMoeExperts + 1) * 4 + 1024 <= 227 * 1024, "shared memory plan");
+};
+
+__device__ __forceinline__ void tmem_alloc(uint32_t *slot, uint32_t ncols) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)),
+                 "r"(ncols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tc_commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+// Four rows of the token matrix, 128 bytes of each from column x.
+__device__ __forceinline__ void tma_gather4(void *dst, const CUtensorMap *map, int x, const int (&r)[4],
+                                            uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+        "%3, %4, %5, %6}], [%7];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(smem_u32(bar))
+        : "memory");
+}
+// 32 lanes x NC columns of 32 bits, lane quarter in the address's upper half.
+template <int NC>
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&v)[NC]) {
+    static_assert(NC == 16 || NC == 32, "16 or 32 columns");
+    if constexpr (NC == 32) {
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+            "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+            : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+              "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+              "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+              "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+            : "r"(taddr));
+    } else {
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+            "%15}, [%16];"
+            : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+              "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+            : "r"(taddr));
+    }
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+// K-major operand, 128-byte swizzle, 8-row groups 1024 bytes apart, version 1.
+__device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// kind::i8: s32 accumulator (2 at bit 4), signed A and B (1 at bits 7 and 10), N>>3 at 17, M>>4 at 24.
+__device__ __forceinline__ uint32_t idesc_for(int n) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(BN >> 4) << 24);
+}
+
+__device__ __forceinline__ bool wait_s8(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
+    const uint32_t b = smem_u32(bar);
+    if (mbar_try_wait(b, parity)) return true;
+    const unsigned long long t0 = global_ns();
+    while (!mbar_try_wait(b, parity)) {
+        if (*abort_flag) return false;
+        if (global_ns() - t0 > kWaitLimitNs) {
+            *abort_flag = 1;
+            atomicExch(&g_s8_timeout, 1u);
+            return false;
+        }
+    }
+    return true;
+}
+
+// A tile: rows [row0, row0 + rows) of C (and of A, unless gathered), channels from n0 of expert e.
+struct Tile {
+    int e, row0, rows, n0;
+};
+
+__device__ __forceinline__ int round16(int v) { return (v + 15) & ~15; }
+
+// Tile t.  Grouped: first[e] tiles before expert e, off[e] its first row; the offsets come from
+// device memory and were clamped to [0, M] and to ascending order when they were read.
+template <int MODE>
+__device__ __forceinline__ Tile tile_of(const Args &a, int t, const int *first, const int *off) {
+    Tile r;
+    int lo = 0, row_begin = 0, row_end = a.M, q = t;
+    if constexpr (MODE != kDense) {
+        int hi = a.E;  // the last expert with first[e] <= t has tile t (first[e + 1] > t)
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (first[mid] <= t) lo = mid;
+            else hi = mid;
+        }
+        row_begin = off[lo];
+        row_end = off[lo + 1];
+        q = t - first[lo];
+    }
+    const int mt = (row_end - row_begin + a.bt - 1) / a.bt;
+    r.e = lo;
+    r.n0 = q / mt * BN;
+    r.row0 = row_begin + q % mt * a.bt;
+    r.rows = min(a.bt, row_end - r.row0);
+    return r;
+}
+
+__device__ __forceinline__ void store_c(const Args &a, size_t o, float v) { store_out(a.c, a.c_dtype, o, v); }
+
+template <int BT, int MODE>
+__global__ void __launch_bounds__(kThreads, 1)
+s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap a_map, const Args a) {
+    using C_ = Cfg<BT>;
+    constexpr int S = C_::S;
+    extern __shared__ uint8_t smem_dyn[];
+    uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
+    uint64_t *full = reinterpret_cast<uint64_t *>(sm + C_::BAR_OFF);
+    uint64_t *empty = full + S;
+    uint64_t *acc_full = empty + S;  // [2]
+    uint64_t *acc_empty = acc_full + 2;
+    uint64_t *drain = acc_empty + 2;
+    float *as_sh = reinterpret_cast<float *>(sm + C_::AS_OFF);  // [2][BT] token scales
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sm + C_::MISC_OFF);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(sm + C_::MISC_OFF + 4);
+    int *first = reinterpret_cast<int *>(sm + C_::TILE_OFF);  // [E + 1] tiles before each expert
+    int *off = first + a.E + 1;                                // [E + 1] its first row
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int nkb_all = (a.K + BK - 1) / BK;
+    // K split over the cluster (grid z): this CTA sums blocks [kb0, kb1) of its one tile
+    const int ks = gridDim.z, kr = blockIdx.z;
+    const int kb0 = (int)((long)nkb_all * kr / ks), kb1 = (int)((long)nkb_all * (kr + 1) / ks);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&acc_full[i], 1);
+            mbar_init(&acc_empty[i], kEpi);
+        }
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        fence_mbar_init();
+        prefetch_tensormap(&w_map);
+        prefetch_tensormap(&a_map);
+    }
+    if (warp == 1) tmem_alloc(tmem_slot, C_::TMEM_COLS);
+    grid_dep_launch();
+    grid_dep_wait();
+    int ntiles;
+    if constexpr (MODE == kDense) {
+        ntiles = (a.M + a.bt - 1) / a.bt * a.ntn;
+    } else {
+        if (warp == 0) {  // prefix over the experts, 32 at a time
+            int tiles = 0, row = min(max(a.offsets[0], 0), a.M);
+            for (int e0 = 0; e0 < a.E; e0 += 32) {
+                const int e = e0 + lane;
+                int end = e < a.E ? min(max(a.offsets[e + 1], 0), a.M) : 0;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {  // ascending whatever the memory holds
+                    const int u = __shfl_up_sync(0xffffffffu, end, o);
+                    if (lane >= o) end = max(end, u);
+                }
+                end = max(end, row);
+                int begin = __shfl_up_sync(0xffffffffu, end, 1);
+                if (lane == 0) begin = row;
+                int n = e < a.E ? (end - begin + a.bt - 1) / a.bt * a.ntn : 0;
+                int inc = n;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int u = __shfl_up_sync(0xffffffffu, inc, o);
+                    if (lane >= o) inc += u;
+                }
+                if (e < a.E) {
+                    first[e] = tiles + inc - n;
+                    off[e] = begin;
+                    if (e == a.E - 1) {
+                        first[a.E] = tiles + inc;
+                        off[a.E] = end;
+                    }
+                }
+                tiles += __shfl_sync(0xffffffffu, inc, 31);
+                row = __shfl_sync(0xffffffffu, end, 31);
+            }
+        }
+        ntiles = 0;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if constexpr (MODE != kDense) ntiles = first[a.E];
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0) {
+        // ---------------- producer ----------------
+        int g = 0;  // k-blocks issued (stage g % S)
+        bool ok = true;
+        for (int t = blockIdx.x; t < ntiles && ok; t += gridDim.x) {
+            const Tile tl = tile_of<MODE>(a, t, first, off);
+            const int need = round16(tl.rows);
+            const int boxes = (need + a.box - 1) / a.box;
+            const uint32_t tx = W_BYTES + (uint32_t)(MODE == kGathered ? need : boxes * a.box) * BK;
+            int idx[(BT + 127) / 128][4];  // gathered: this lane's rows
+            if constexpr (MODE == kGathered) {
+#pragma unroll
+                for (int i = 0; i < (BT + 127) / 128; ++i)
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const int r = (i * 32 + lane) * 4 + u;
+                        idx[i][u] = r < tl.rows ? a.src[tl.row0 + r] : -1;
+                        if (idx[i][u] < 0 || idx[i][u] >= a.a_rows) idx[i][u] = 0;  // scaled by 0, or not stored
+                    }
+            }
+            for (int kb = kb0; kb < kb1; ++kb, ++g) {
+                const int s = g % S;
+                if (g >= S && !__all_sync(0xffffffffu, wait_s8(&empty[s], (uint32_t)((g / S - 1) & 1), abort_flag))) {
+                    ok = false;
+                    break;
+                }
+                uint8_t *w_dst = sm + s * C_::STAGE, *t_dst = w_dst + W_BYTES;
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(&full[s], tx);
+                    tma_load_3d(w_dst, &w_map, kb * BK, tl.n0, tl.e, &full[s]);
+                    if constexpr (MODE != kGathered)
+                        for (int b = 0; b < boxes; ++b)
+                            tma_load_2d(t_dst + b * a.box * BK, &a_map, kb * BK, tl.row0 + b * a.box, &full[s]);
+                }
+                if constexpr (MODE == kGathered) {
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < (BT + 127) / 128; ++i)
+                        if ((i * 32 + lane) * 4 < need)
+                            tma_gather4(t_dst + (i * 32 + lane) * 4 * BK, &a_map, kb * BK, idx[i], &full[s]);
+                }
+            }
+        }
+        // after a wait that gave up, nothing of this CTA's copies may still be in flight at its end
+        if (*abort_flag)
+            for (int i = g > S ? g - S : 0; i < g; ++i) mbar_wait_bounded(&full[i % S], (uint32_t)((i / S) & 1));
+    } else if (warp == 1) {
+        // ---------------- MMA issuer ----------------
+        if (lane == 0) {
+            const uint64_t d0 = sw128_desc(smem_u32(sm));
+            int g = 0, j = 0;
+            bool ok = true;
+            for (int t = blockIdx.x; t < ntiles && ok; t += gridDim.x, ++j) {
+                const Tile tl = tile_of<MODE>(a, t, first, off);
+                const uint32_t idesc = idesc_for(round16(tl.rows));
+                const uint32_t acc = tmem + (uint32_t)(j & 1) * BT;
+                if (j >= 2 && !wait_s8(&acc_empty[j & 1], (uint32_t)((j / 2 - 1) & 1), abort_flag)) break;
+                tc_fence_after();
+                for (int kb = kb0; kb < kb1; ++kb, ++g) {
+                    const int s = g % S;
+                    if (!wait_s8(&full[s], (uint32_t)((g / S) & 1), abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint64_t wd = d0 + (uint64_t)(s * (C_::STAGE >> 4)), td = wd + (W_BYTES >> 4);
+                    const int steps = min(4, (a.K - kb * BK + 31) / 32);  // 32 k a step
+                    for (int kk = 0; kk < steps; ++kk)
+                        mma_i8(acc, wd + 2 * kk, td + 2 * kk, idesc, kb > kb0 || kk > 0);
+                    tc_commit(&empty[s]);
+                }
+                if (!ok) break;
+                tc_commit(&acc_full[j & 1]);
+            }
+            if (*abort_flag) {  // let the MMAs in flight end before TMEM is freed
+                tc_commit(drain);
+                mbar_wait_bounded(drain, 0u);
+            }
+        }
+    } else {
+        // ---------------- epilogue: lane quarter warp % 4 ----------------
+        const int q = warp & 3, et = threadIdx.x - 64;
+        int j = 0;
+        for (int t = blockIdx.x; t < ntiles; t += gridDim.x, ++j) {
+            const Tile tl = tile_of<MODE>(a, t, first, off);
+            float *as = as_sh + (j & 1) * BT;
+            for (int i = et; i < tl.rows; i += kEpi * 32) {
+                int r = tl.row0 + i;
+                if constexpr (MODE == kGathered) r = a.src[r];
+                as[i] = MODE != kGathered || (r >= 0 && r < a.a_rows) ? a.a_scale[r] : 0.f;
+            }
+            const int n = tl.n0 + 32 * q + lane;
+            const bool in = n < a.N;
+            const float ws = in ? a.w_scale[(size_t)tl.e * a.N + n] : 0.f;
+            const float bs = in && a.bias ? a.bias[(size_t)tl.e * a.N + n] : 0.f;
+            asm volatile("bar.sync 1, %0;" ::"r"(kEpi * 32) : "memory");  // as[] is complete
+            if (!__all_sync(0xffffffffu, wait_s8(&acc_full[j & 1], (uint32_t)((j / 2) & 1), abort_flag))) break;
+            tc_fence_after();
+            const uint32_t acc = tmem + (uint32_t)(j & 1) * BT + ((uint32_t)(32 * q) << 16);
+            for (int c0 = 0; c0 < tl.rows; c0 += C_::LD) {
+                uint32_t v[C_::LD];
+                tmem_ld<C_::LD>(acc + c0, v);
+                if (ks > 1) {  // raw sums, summed over the cluster below
+                    int *red = reinterpret_cast<int *>(sm) + c0 * BN + 32 * q + lane;
+#pragma unroll
+                    for (int i = 0; i < (int)C_::LD; ++i) red[i * BN] = (int)v[i];
+                } else if (in) {
+#pragma unroll
+                    for (int i = 0; i < (int)C_::LD; ++i)
+                        if (c0 + i < tl.rows)
+                            store_c(a, (size_t)(tl.row0 + c0 + i) * a.N + n,
+                                    fmaf((float)(int)v[i] * as[c0 + i], ws, bs));
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[j & 1]);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, C_::TMEM_COLS);
+    }
+    if (ks > 1) {
+        // Every CTA of the cluster holds its part of one tile's sums (s32: the order does not
+        // matter) where its stages were; each finishes an equal share of the tile.
+        cluster_sync_all();
+        if ((int)blockIdx.x < ntiles) {
+            const Tile tl = tile_of<MODE>(a, blockIdx.x, first, off);
+            const int total = tl.rows * BN;
+            const int i1 = (int)((long)total * (kr + 1) / ks);
+            for (int i = (int)((long)total * kr / ks) + threadIdx.x; i < i1; i += kThreads) {
+                const int row = i / BN, n = tl.n0 + i % BN;
+                int sum = 0;
+                for (int r = 0; r < ks; ++r)
+                    sum += __float_as_int(ld_cluster_f32(reinterpret_cast<const float *>(sm) + i, (uint32_t)r));
+                if (n < a.N)
+                    store_c(a, (size_t)(tl.row0 + row) * a.N + n,
+                            fmaf((float)sum * as_sh[row], a.w_scale[(size_t)tl.e * a.N + n],
+                                 a.bias ? a.bias[(size_t)tl.e * a.N + n] : 0.f));
+            }
+        }
+        cluster_sync_all();  // nobody leaves while its sums are read
+    }
+}
+
+template <int BT, int MODE>
+static int launch(const CUtensorMap &w_map, const CUtensorMap &a_map, const Args &a, int grid, int ks,
+                  cudaStream_t st) {
+    const size_t smem = Cfg<BT>::smem(MODE == kDense ? 0 : a.E);
+    auto kern = s8_gemm_kernel<BT, MODE>;
+    W4_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    W4_CUDA_TRY(launch_decode(kern, dim3(grid, 1, ks), dim3(kThreads), smem, st, ks, w_map, a_map, a));
+    return W4_OK;
+}
+
+template <int MODE>
+static int launch_bt(int BT, const CUtensorMap &w_map, const CUtensorMap &a_map, const Args &a, int grid, int ks,
+                     cudaStream_t st) {
+    switch (BT) {
+        case 16: return launch<16, MODE>(w_map, a_map, a, grid, ks, st);
+        case 64: return launch<64, MODE>(w_map, a_map, a, grid, ks, st);
+        case 128: return launch<128, MODE>(w_map, a_map, a, grid, ks, st);
+        default: return launch<256, MODE>(w_map, a_map, a, grid, ks, st);
+    }
+}
+
+static int capacity_for(int rows) { return rows <= 16 ? 16 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256; }
+
+static int map_failed() {
+    set_error("s8 GEMM: the tensor map of an operand was refused (shape or alignment)");
+    return W4_ERR_UNSUPPORTED;
+}
+
+}  // namespace s8g
+
+int s8_gemm(const int8_t *a, const float *a_scale, const int8_t *w, const float *w_scale, const float *bias, void *c,
+            int c_dtype, int M, int N, int K, cudaStream_t st) {
+    using namespace s8g;
+    Args g = {a_scale, w_scale, bias, nullptr, nullptr, c, c_dtype, M, M, N, K, 1, 0, 0, (N + BN - 1) / BN};
+    const int BT = capacity_for(M);
+    const int mt = (M + BT - 1) / BT;
+    g.bt = ((M + mt - 1) / mt + 15) / 16 * 16;  // equal tiles of rows
+    g.box = g.bt;
+    CUtensorMap w_map, a_map;
+    if (!make_map_3d(&w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, w, K, N, 1, K, (uint64_t)N * K, BK, BN,
+                     CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !make_map_2d(&a_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, a, K, M, K, BK, g.box, CU_TENSOR_MAP_SWIZZLE_128B))
+        return map_failed();
+    const long tiles = (long)((M + g.bt - 1) / g.bt) * g.ntn;
+    W4_REQUIRE(tiles < (1L << 30), W4_ERR_UNSUPPORTED, "s8 GEMM: %ld tiles", tiles);
+    // Few tiles: a cluster splits K, at least four blocks to a CTA.
+    int ks = 1;
+    const int nsm = num_sms(), nkb = (K + BK - 1) / BK;
+    if (2 * tiles <= nsm && BT <= 128) {
+        ks = (int)(nsm / tiles);
+        ks = ks > 8 ? 8 : ks;
+        ks = ks > nkb / 4 ? nkb / 4 : ks;
+        ks = ks < 1 ? 1 : ks;
+    }
+    return launch_bt<kDense>(BT, w_map, a_map, g, (int)(tiles < nsm ? tiles : nsm), ks, st);
+}
+
+int s8_gemm_grouped(const int8_t *a, int a_rows, const float *a_scale, const int8_t *w, const float *w_scale,
+                    const float *bias, const int *offsets, const int *src, int E, void *c, int c_dtype, int R, int N,
+                    int K, cudaStream_t st) {
+    using namespace s8g;
+    Args g = {a_scale, w_scale, bias, offsets, src, c, c_dtype, R, a_rows, N, K, E, 0, 0, (N + BN - 1) / BN};
+    // The counts are on the device: capacity for about twice the average expert's rows.
+    const int BT = capacity_for((int)(2L * R / E));
+    g.bt = BT;
+    g.box = BT < 32 ? BT : 32;
+    CUtensorMap w_map, a_map;
+    if (!make_map_3d(&w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, w, K, N, E, K, (uint64_t)N * K, BK, BN,
+                     CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !make_map_2d(&a_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, a, K, a_rows, K, BK, src ? 1 : g.box,
+                     CU_TENSOR_MAP_SWIZZLE_128B))
+        return map_failed();
+    const long most = ((long)R / g.bt + (R < E ? R : E)) * g.ntn;  // tiles at most, whatever the counts
+    W4_REQUIRE(most < (1L << 30), W4_ERR_UNSUPPORTED, "s8 GEMM: %ld tiles", most);
+    const int grid = (int)(most < num_sms() ? most : num_sms());
+    return src ? launch_bt<kGathered>(BT, w_map, a_map, g, grid, 1, st)
+               : launch_bt<kGrouped>(BT, w_map, a_map, g, grid, 1, st);
+}
+
+int take_s8_wait_status() {
+    unsigned int v = 0;
+    W4_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_s8_timeout, sizeof(v)));
+    if (v) {
+        const unsigned int zero = 0;
+        W4_CUDA_TRY(cudaMemcpyToSymbol(g_s8_timeout, &zero, sizeof(zero)));
+        set_error("a device-side wait expired in the s8 GEMM");
+        return W4_ERR_TIMEOUT;
+    }
+    return W4_OK;
+}
+
+}  // namespace w4

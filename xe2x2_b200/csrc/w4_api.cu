@@ -95,7 +95,8 @@ int w4_check_device_status(void) {
     const int r6 = w4::take_tp_fused_wait_status();
     const int r7 = w4::take_rn_wait_status();
     const int r8 = w4::take_decode_wait_status();
-    return r1 ? r1 : r2 ? r2 : r3 ? r3 : r4 ? r4 : r5 ? r5 : r6 ? r6 : r7 ? r7 : r8;
+    const int r9 = w4::take_s8_wait_status();
+    return r1 ? r1 : r2 ? r2 : r3 ? r3 : r4 ? r4 : r5 ? r5 : r6 ? r6 : r7 ? r7 : r8 ? r8 : r9;
 }
 
 // ------------------------------------------------------------------ GPTQ
@@ -634,6 +635,74 @@ int w4_quant_s8(const void *x, int x_dtype, int fn, int8_t *q, float *scale, int
     W4_REQUIRE(aligned(x, 16) && aligned(q, 16) && aligned(scale, 4), W4_ERR_INVALID,
                "x and q must be 16-byte aligned, scale 4-byte");
     return w4::quant_s8(x, x_dtype, fn, q, scale, M, K, S(stream));
+}
+
+size_t w4_s8_gemm_workspace_bytes(int M, int N, int K, int c_dtype) {
+    if (M <= 0 || N <= 0 || K <= 0 || c_dtype != W4_E4M3) return 0;
+    return align256((size_t)M * N * 4);
+}
+
+// The argument rules that the plain and the grouped s8 GEMM share (rows > 0).
+static int check_s8(const int8_t *a, const float *a_scale, const int8_t *w, const float *w_scale, const float *bias,
+                    const void *c, int c_dtype, const float *row_scale, int rows, int N, int K, const void *workspace,
+                    size_t workspace_bytes) {
+    W4_REQUIRE(a && a_scale && w && w_scale && c, W4_ERR_INVALID, "a, a_scale, w, w_scale and c are required");
+    W4_REQUIRE(c_dtype != W4_E4M3 || row_scale, W4_ERR_INVALID, "e4m3 output needs row_scale");
+    W4_REQUIRE(aligned(a, 16) && aligned(w, 16) && aligned(a_scale, 4) && aligned(w_scale, 4) && aligned(bias, 4) &&
+                   aligned(row_scale, 4) && aligned(c, c_dtype == W4_F32 ? 4 : c_dtype == W4_E4M3 ? 1 : 2),
+               W4_ERR_INVALID, "a and w must be 16-byte aligned, the others to their element size");
+    const size_t need = w4_s8_gemm_workspace_bytes(rows, N, K, c_dtype);
+    W4_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 16)), W4_ERR_INVALID,
+               "a 16-byte aligned workspace of %zu bytes is needed (%zu given)", need, workspace_bytes);
+    return W4_OK;
+}
+
+static int check_s8_shape(int c_dtype, int rows, int N, int K) {
+    W4_REQUIRE(float_dtype(c_dtype) || c_dtype == W4_E4M3, W4_ERR_INVALID, "c_dtype must be f16, bf16, f32 or e4m3");
+    W4_REQUIRE(rows >= 0 && N >= 1 && K >= 1, W4_ERR_INVALID, "rows=%d N=%d K=%d", rows, N, K);
+    W4_REQUIRE(K % 16 == 0 && K <= 131056, W4_ERR_UNSUPPORTED, "K=%d must be a multiple of 16, at most 131056", K);
+    return W4_OK;
+}
+
+int w4_s8_gemm(const int8_t *a, const float *a_scale, const int8_t *w, const float *w_scale, const float *bias,
+               void *c, int c_dtype, float *row_scale, int M, int N, int K, void *workspace,
+               size_t workspace_bytes, void *stream) {
+    w4::set_error("");
+    int rc = check_s8_shape(c_dtype, M, N, K);
+    if (rc || M == 0) return rc;
+    rc = check_s8(a, a_scale, w, w_scale, bias, c, c_dtype, row_scale, M, N, K, workspace, workspace_bytes);
+    if (rc) return rc;
+    if (c_dtype != W4_E4M3) return w4::s8_gemm(a, a_scale, w, w_scale, bias, c, c_dtype, M, N, K, S(stream));
+    rc = w4::s8_gemm(a, a_scale, w, w_scale, bias, workspace, W4_F32, M, N, K, S(stream));
+    return rc ? rc
+              : w4::rowscale_fp8(workspace, W4_F32, static_cast<uint8_t *>(c), row_scale, M, N, S(stream));
+}
+
+size_t w4_s8_gemm_grouped_workspace_bytes(int R, int N, int K, int c_dtype) {
+    return w4_s8_gemm_workspace_bytes(R, N, K, c_dtype);
+}
+
+int w4_s8_gemm_grouped(const int8_t *a, const float *a_scale, int a_rows, const int8_t *w, const float *w_scale,
+                       const float *bias, const int32_t *offsets, const int32_t *rows, int E, void *c, int c_dtype,
+                       float *row_scale, int R, int N, int K, void *workspace, size_t workspace_bytes,
+                       void *stream) {
+    w4::set_error("");
+    int rc = check_s8_shape(c_dtype, R, N, K);
+    if (rc) return rc;
+    W4_REQUIRE(E >= 1, W4_ERR_INVALID, "E=%d", E);
+    W4_REQUIRE(E <= w4::kMaxMoeExperts, W4_ERR_UNSUPPORTED, "E=%d exceeds %d experts", E, w4::kMaxMoeExperts);
+    W4_REQUIRE(a_rows >= 0 && (rows || a_rows == R), W4_ERR_INVALID, "a_rows=%d must be R=%d without rows", a_rows, R);
+    if (R == 0) return W4_OK;
+    W4_REQUIRE(a_rows >= 1, W4_ERR_INVALID, "a has no rows to gather from");
+    W4_REQUIRE(offsets && aligned(offsets, 4) && aligned(rows, 4), W4_ERR_INVALID,
+               "offsets are required, offsets and rows 4-byte aligned");
+    rc = check_s8(a, a_scale, w, w_scale, bias, c, c_dtype, row_scale, R, N, K, workspace, workspace_bytes);
+    if (rc) return rc;
+    void *out = c_dtype == W4_E4M3 ? workspace : c;
+    rc = w4::s8_gemm_grouped(a, a_rows, a_scale, w, w_scale, bias, offsets, rows, E, out,
+                             c_dtype == W4_E4M3 ? W4_F32 : c_dtype, R, N, K, S(stream));
+    if (rc || c_dtype != W4_E4M3) return rc;
+    return w4::rowscale_fp8(out, W4_F32, static_cast<uint8_t *>(c), row_scale, R, N, S(stream), offsets + E);
 }
 
 size_t w4_moe_route_workspace_bytes(int T, int E) {

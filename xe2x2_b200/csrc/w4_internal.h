@@ -153,8 +153,9 @@ int nvfp4_prefill_q(const uint8_t *codes, const uint8_t *sfa, const float *a_glo
 size_t nvfp4_prefill_q_workspace(int M, int N, int K, bool scale_atoms_needed);
 // C = sum over splits of the fp32 partials [splits][mn] (mn % 4 == 0), in c_dtype (gptq_prefill.cu).
 int splitk_reduce(const float *partial, int splits, long mn, void *c, int c_dtype, cudaStream_t st);
+// limit (device, or null): rows from *limit on are left alone
 int rowscale_fp8(const void *y, int y_dtype, uint8_t *q, float *row_scale, int M, int N,
-                 cudaStream_t st);
+                 cudaStream_t st, const int *limit = nullptr);
 // The same cast (bit for bit) from f32 y whose row maxima a decode GEMM folded into rowmax (fp32
 // bits, M <= 16); the last CTA of each row zeroes rowmax[row] again, counting on rowcnt[row].
 int rowscale_fp8_amax(const float *y, unsigned int *rowmax, unsigned int *rowcnt, uint8_t *q, float *row_scale,
@@ -162,6 +163,15 @@ int rowscale_fp8_amax(const float *y, unsigned int *rowmax, unsigned int *rowcnt
 
 // s8_quant.cu: per-token s8 quantisation of fn(x) (W4_FN_*)
 int quant_s8(const void *x, int x_dtype, int fn, int8_t *q, float *scale, int M, int K, cudaStream_t st);
+
+// s8_gemm.cu: W8A8 GEMM, plain and over a batch sorted by expert (device offsets); c_dtype f16,
+// bf16 or f32
+int s8_gemm(const int8_t *a, const float *a_scale, const int8_t *w, const float *w_scale, const float *bias, void *c,
+            int c_dtype, int M, int N, int K, cudaStream_t st);
+int s8_gemm_grouped(const int8_t *a, int a_rows, const float *a_scale, const int8_t *w, const float *w_scale,
+                    const float *bias, const int *offsets, const int *src, int E, void *c, int c_dtype, int R, int N,
+                    int K, cudaStream_t st);
+int take_s8_wait_status();
 
 // moe.cu: the router with the batch's order by expert, and the weighted sum of expert outputs
 constexpr int kMaxTopK = 32, kMaxGroups = 32, kMaxMoeExperts = 512;

@@ -439,6 +439,95 @@ def quant_s8(x, act=None):
     return q, s
 
 
+_S8_OUT = {**_FLOATS, torch.float8_e4m3fn: L.W4_E4M3}
+
+
+def _s8_out(M, N, out_dtype, out, dev):
+    """Output tensor, row scales and scratch of an s8 GEMM.  The scratch is allocated by the call, so
+    no two streams or captured graphs share it."""
+    out_dtype = out_dtype or (out.dtype if out is not None else torch.bfloat16)
+    if out_dtype not in _S8_OUT:
+        raise ValueError(f"out_dtype must be f16, bf16, f32 or float8_e4m3fn, got {out_dtype}")
+    if out is None:
+        out = torch.empty((M, N), dtype=out_dtype, device=dev)
+    else:
+        _tensor(out, "out", out_dtype, (M, N), dev)
+    rs = ws = None
+    need = 0
+    if out_dtype == torch.float8_e4m3fn:
+        rs = torch.empty(M, dtype=torch.float32, device=dev)
+        need = L.lib().w4_s8_gemm_workspace_bytes(M, N, 16, L.W4_E4M3)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    return out, _S8_OUT[out_dtype], rs, ws, need
+
+
+def s8_gemm(a, a_scale, w, w_scale, bias=None, out_dtype=None, out=None):
+    """W8A8 GEMM: (a s8 [M, K] . w s8 [N, K]^T) * a_scale[M] * w_scale[N] + bias[N] -> [M, N].
+
+    ``a``, ``a_scale`` from :func:`quant_s8` or :func:`rmsnorm_quant_s8`; scales and bias f32.
+    K a multiple of 16 (at most 131056), any M and N.  ``out_dtype``: f16, bf16 (default), f32, or
+    float8_e4m3fn, which applies the per-row fp8 cast and also returns the f32 row scales.  ``out``
+    (optional) receives the result in place.
+    """
+    if not torch.is_tensor(a) or a.dim() != 2 or not torch.is_tensor(w) or w.dim() != 2:
+        raise ValueError("a must be [M, K] and w [N, K]")
+    dev = a.device
+    (M, K), N = a.shape, w.shape[0]
+    _tensor(a, "a", torch.int8, (M, K), dev)
+    _tensor(a_scale, "a_scale", torch.float32, (M,), dev)
+    _tensor(w, "w", torch.int8, (N, K), dev)
+    _tensor(w_scale, "w_scale", torch.float32, (N,), dev)
+    _tensor(bias, "bias", torch.float32, (N,), dev, optional=True)
+    c, cdt, rs, ws, need = _s8_out(M, N, out_dtype, out, dev)
+    _call_on(dev, "w4_s8_gemm", _p(a), _p(a_scale), _p(w), _p(w_scale), _p(bias), _p(c), cdt, _p(rs), M, N, K, _p(ws),
+             need)
+    return c if rs is None else (c, rs)
+
+
+def s8_gemm_grouped(a, a_scale, w, w_scale, offsets, rows=None, bias=None, out_dtype=None, out=None):
+    """Grouped (MoE) W8A8 GEMM in one launch: expert e multiplies rows [offsets[e], offsets[e + 1]) of
+    the batch by w[e] (w s8 [E, N, K], w_scale and bias f32 [E, N]).
+
+    ``offsets``: i32 [E + 1] on the device (:func:`moe_route`), never read by the host.  ``rows``:
+    i32 [R] on the device; row r of the batch is then row rows[r] of ``a`` [tokens, K] with its scale,
+    so tokens are quantised once and never copied.  Without it ``a`` is the batch, [R, K].
+    Returns [R, N] (types as :func:`s8_gemm`); rows behind offsets[E] are not written.
+    """
+    if not torch.is_tensor(a) or a.dim() != 2 or not torch.is_tensor(w) or w.dim() != 3:
+        raise ValueError("a must be [tokens, K] and w [E, N, K]")
+    dev = a.device
+    (A, K), (E, N) = a.shape, w.shape[:2]
+    _tensor(a, "a", torch.int8, (A, K), dev)
+    _tensor(a_scale, "a_scale", torch.float32, (A,), dev)
+    _tensor(w, "w", torch.int8, (E, N, K), dev)
+    _tensor(w_scale, "w_scale", torch.float32, (E, N), dev)
+    _tensor(bias, "bias", torch.float32, (E, N), dev, optional=True)
+    _tensor(offsets, "offsets", torch.int32, (E + 1,), dev)
+    R = A
+    if rows is not None:
+        if not torch.is_tensor(rows) or rows.dim() != 1:
+            raise ValueError("rows must be a 1-D tensor")
+        R = rows.shape[0]
+        _tensor(rows, "rows", torch.int32, (R,), dev)
+    c, cdt, rs, ws, need = _s8_out(R, N, out_dtype, out, dev)
+    _call_on(dev, "w4_s8_gemm_grouped", _p(a), _p(a_scale), A, _p(w), _p(w_scale), _p(bias), _p(offsets), _p(rows), E,
+             _p(c), cdt, _p(rs), R, N, K, _p(ws), need)
+    return c if rs is None else (c, rs)
+
+
+class S8Linear:
+    """A W8A8 linear layer: weight s8 [N, K], its per-channel scale f32 [N], bias f32 [N] or None.
+    Calling it quantises the tokens (after ``act``, see :func:`quant_s8`) and multiplies."""
+
+    def __init__(self, weight, weight_scale, bias=None, act=None):
+        self.weight, self.weight_scale, self.bias, self.act = weight, weight_scale, bias, act
+        self.N, self.K = weight.shape
+
+    def __call__(self, x, out_dtype=None):
+        q, s = quant_s8(x, self.act)
+        return s8_gemm(q, s, self.weight, self.weight_scale, self.bias, out_dtype or x.dtype)
+
+
 # ===================================================================== MoE: router, combine
 class MoERouting(NamedTuple):
     """What :func:`moe_route` returns.  ``ids`` i32 [T, k] (best first, -1: none), ``weights`` f32
@@ -514,6 +603,29 @@ def moe_combine(y, slots, weights, add=None, out_dtype=None):
     _call_on(dev, "w4_moe_combine", _p(y), _FLOATS[y.dtype], rows, _p(slots), _p(weights), _p(add), _p(out),
              _FLOATS[out_dtype], T, k, H)
     return out
+
+
+class S8Experts:
+    """The experts of a MoE layer in 8 bits: w_in s8 [E, F, H] (F = 2I for ``act="silu_mul"``, gate
+    rows before up rows; I otherwise), w_out s8 [E, H, I], per-channel scales f32 [E, F] and [E, H].
+
+    Calling it with token states [T, H] and router logits [T, E] routes (``route``: keyword
+    arguments of :func:`moe_route`), quantises each token once, runs both products over the batch
+    sorted by expert and sums each token's outputs, plus ``add``.  Nothing is read back by the
+    host, so a call can be captured into a CUDA graph.
+    """
+
+    def __init__(self, w_in, in_scale, w_out, out_scale, top_k, act="silu_mul", **route):
+        self.w_in, self.in_scale, self.w_out, self.out_scale = w_in, in_scale, w_out, out_scale
+        self.top_k, self.act, self.route = top_k, act, route
+
+    def __call__(self, x, logits, add=None):
+        r = moe_route(logits, self.top_k, **self.route)
+        q, s = quant_s8(x)
+        h = s8_gemm_grouped(q, s, self.w_in, self.in_scale, r.offsets, r.rows, out_dtype=x.dtype)
+        q, s = quant_s8(h, self.act)
+        y = s8_gemm_grouped(q, s, self.w_out, self.out_scale, r.offsets, out_dtype=x.dtype)
+        return moe_combine(y, r.slots, r.weights, add, out_dtype=x.dtype)
 
 
 # ===================================================================== torch.ops.w4
