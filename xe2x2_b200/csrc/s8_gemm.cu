@@ -8,9 +8,11 @@
 // The weights are the MMA's M side (128 output channels a tile) and the tokens its N side, so that
 // one kernel serves every batch: N is 16 for a decode step and 256 for a prompt, and the MMA's N
 // follows the rows that a tile has.  Both operands are K-major 128-byte lines, 128-byte swizzle,
-// fetched by TMA; K is padded with zeros by the copy itself.  Token rows may be gathered through an
-// index (tile::gather4, four rows a copy).  Warp 0 produces, warp 1 issues the MMAs, warps 2-5 read
-// the sums out of TMEM (two accumulators: one fills while the other is read), scale and store.
+// fetched by TMA; K is padded with zeros by the copy itself.  Warp 0 produces, warp 1 issues the
+// MMAs, warps 2-5 read the sums out of TMEM (two accumulators: one fills while the other is read),
+// scale and store.  Token rows that are gathered through an index come by 16-byte cp.async from
+// four more warps: TMA's tile::gather4 (four rows a copy) took 55 to 75 cycles a copy, which made a
+// batch of 4096 tokens x 6 experts (K 2688, N 3712, 64 experts) 1.12 ms against 0.34 ms.
 // Every wait is bounded; no copy names more than one CTA.
 #include <mutex>
 
@@ -25,12 +27,14 @@ static __device__ unsigned int g_s8_timeout;  // a bounded wait expired (sticky 
 namespace s8g {
 
 constexpr int BN = 128, BK = 128;  // output channels and bytes of K in a stage
-constexpr int kThreads = 6 * 32, kEpi = 4;
+constexpr int kEpi = 4, kGather = 4;  // epilogue and gather warps (2-5 and 6-9)
 constexpr uint32_t W_BYTES = BN * BK;
 
 enum Mode { kDense = 0, kGrouped = 1, kGathered = 2 };
+constexpr int threads_of(int mode) { return 32 * (2 + kEpi + (mode == kGathered ? kGather : 0)); }
 
 struct Args {
+    const int8_t *a;  // gathered rows only (TMA has its map)
     const float *a_scale, *w_scale, *bias;
     const int *offsets, *src;
     void *c;
@@ -47,6 +51,7 @@ template <int BT> struct Cfg {
     static constexpr uint32_t BAR_OFF = S * STAGE, AS_OFF = BAR_OFF + (2 * S + 5) * 8 / 16 * 16 + 16,
                               MISC_OFF = AS_OFF + 2 * BT * 4, TILE_OFF = MISC_OFF + 16;
     static constexpr uint32_t LD = BT < 32 ? BT : 32;  // columns of one TMEM read
+    static constexpr int LAG = S / 2;  // stages that a gather warp's copies may be in flight
     static constexpr size_t smem(int E) { return TILE_OFF + (size_t)2 * (E + 1) * 4 + 1024; }
     static_assert(TILE_OFF + 2 * (kMaxMoeExperts + 1) * 4 + 1024 <= 227 * 1024, "shared memory plan");
 };
@@ -76,14 +81,9 @@ __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint3
         "l"(a), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
-// Four rows of the token matrix, 128 bytes of each from column x.
-__device__ __forceinline__ void tma_gather4(void *dst, const CUtensorMap *map, int x, const int (&r)[4],
-                                            uint64_t *bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
-        "%3, %4, %5, %6}], [%7];" ::"r"(smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(smem_u32(bar))
-        : "memory");
+// 16 bytes global -> shared, asynchronously; zeros where n is 0.
+__device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void *src, uint32_t n) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 // 32 lanes x NC columns of 32 bits, lane quarter in the address's upper half.
 template <int NC>
@@ -168,7 +168,7 @@ __device__ __forceinline__ Tile tile_of(const Args &a, int t, const int *first, 
 __device__ __forceinline__ void store_c(const Args &a, size_t o, float v) { store_out(a.c, a.c_dtype, o, v); }
 
 template <int BT, int MODE>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(threads_of(MODE), 1)
 s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap a_map, const Args a) {
     using C_ = Cfg<BT>;
     constexpr int S = C_::S;
@@ -192,7 +192,7 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
-            mbar_init(&full[s], 1);
+            mbar_init(&full[s], MODE == kGathered ? 1 + kGather : 1);
             mbar_init(&empty[s], 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -258,20 +258,8 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
         bool ok = true;
         for (int t = blockIdx.x; t < ntiles && ok; t += gridDim.x) {
             const Tile tl = tile_of<MODE>(a, t, first, off);
-            const int need = round16(tl.rows);
-            const int boxes = (need + a.box - 1) / a.box;
-            const uint32_t tx = W_BYTES + (uint32_t)(MODE == kGathered ? need : boxes * a.box) * BK;
-            int idx[(BT + 127) / 128][4];  // gathered: this lane's rows
-            if constexpr (MODE == kGathered) {
-#pragma unroll
-                for (int i = 0; i < (BT + 127) / 128; ++i)
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const int r = (i * 32 + lane) * 4 + u;
-                        idx[i][u] = r < tl.rows ? a.src[tl.row0 + r] : -1;
-                        if (idx[i][u] < 0 || idx[i][u] >= a.a_rows) idx[i][u] = 0;  // scaled by 0, or not stored
-                    }
-            }
+            const int boxes = MODE == kGathered ? 0 : (round16(tl.rows) + a.box - 1) / a.box;
+            const uint32_t tx = W_BYTES + (uint32_t)(boxes * a.box) * BK;
             for (int kb = kb0; kb < kb1; ++kb, ++g) {
                 const int s = g % S;
                 if (g >= S && !__all_sync(0xffffffffu, wait_s8(&empty[s], (uint32_t)((g / S - 1) & 1), abort_flag))) {
@@ -282,16 +270,8 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
                 if (lane == 0) {
                     mbar_arrive_expect_tx(&full[s], tx);
                     tma_load_3d(w_dst, &w_map, kb * BK, tl.n0, tl.e, &full[s]);
-                    if constexpr (MODE != kGathered)
-                        for (int b = 0; b < boxes; ++b)
-                            tma_load_2d(t_dst + b * a.box * BK, &a_map, kb * BK, tl.row0 + b * a.box, &full[s]);
-                }
-                if constexpr (MODE == kGathered) {
-                    __syncwarp();
-#pragma unroll
-                    for (int i = 0; i < (BT + 127) / 128; ++i)
-                        if ((i * 32 + lane) * 4 < need)
-                            tma_gather4(t_dst + (i * 32 + lane) * 4 * BK, &a_map, kb * BK, idx[i], &full[s]);
+                    for (int b = 0; b < boxes; ++b)
+                        tma_load_2d(t_dst + b * a.box * BK, &a_map, kb * BK, tl.row0 + b * a.box, &full[s]);
                 }
             }
         }
@@ -331,6 +311,50 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
                 mbar_wait_bounded(drain, 0u);
             }
         }
+    } else if (MODE == kGathered && warp >= 2 + kEpi) {
+        // ---------------- gather: token rows through the index, 16 bytes a thread and copy ----------------
+        // Thread (row r0 + 16 i, chunk c): chunk c of row r lies at c ^ (r % 8) of its 128-byte line.
+        // A stage is handed over LAG stages after its copies were issued: each thread waits for its
+        // own, orders them before the tensor core's reads (proxy fence), and lane 0 arrives.
+        constexpr int LAG = C_::LAG, ROWS = kGather * 32 / 8, NR = (BT + ROWS - 1) / ROWS;
+        const int gt = threadIdx.x - 32 * (2 + kEpi), r0 = gt >> 3, c = gt & 7;
+        const uint32_t line = (uint32_t)(r0 * BK + ((c ^ (r0 & 7)) << 4));  // ROWS is a multiple of 8
+        int g = 0;
+        bool ok = true;
+        for (int t = blockIdx.x; t < ntiles && ok; t += gridDim.x) {
+            const Tile tl = tile_of<MODE>(a, t, first, off);
+            const int8_t *row[NR];
+#pragma unroll
+            for (int i = 0; i < NR; ++i) {
+                const int r = r0 + i * ROWS;
+                const int src = r < tl.rows ? a.src[tl.row0 + r] : 0;
+                row[i] = a.a + (size_t)(src >= 0 && src < a.a_rows ? src : 0) * a.K;  // else scaled by 0
+            }
+            for (int kb = kb0; kb < kb1; ++kb, ++g) {
+                const int s = g % S;
+                if (g >= S && !__all_sync(0xffffffffu, wait_s8(&empty[s], (uint32_t)((g / S - 1) & 1), abort_flag))) {
+                    ok = false;
+                    break;
+                }
+                const int x = kb * BK + c * 16;
+                const uint32_t n = x < a.K ? 16u : 0u, dst = smem_u32(sm + s * C_::STAGE + W_BYTES) + line;
+#pragma unroll
+                for (int i = 0; i < NR; ++i)
+                    if (r0 + i * ROWS < tl.rows) cp_async16_zfill(dst + i * ROWS * BK, row[i] + (n ? x : 0), n);
+                cp_async_commit();
+                if (g >= LAG) {
+                    cp_async_wait<LAG>();
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&full[(g - LAG) % S]);
+                }
+            }
+        }
+        cp_async_wait<0>();
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0)
+            for (int i = g > LAG ? g - LAG : 0; i < g; ++i) mbar_arrive(&full[i % S]);
     } else {
         // ---------------- epilogue: lane quarter warp % 4 ----------------
         const int q = warp & 3, et = threadIdx.x - 64;
@@ -385,7 +409,7 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
             const Tile tl = tile_of<MODE>(a, blockIdx.x, first, off);
             const int total = tl.rows * BN;
             const int i1 = (int)((long)total * (kr + 1) / ks);
-            for (int i = (int)((long)total * kr / ks) + threadIdx.x; i < i1; i += kThreads) {
+            for (int i = (int)((long)total * kr / ks) + threadIdx.x; i < i1; i += blockDim.x) {
                 const int row = i / BN, n = tl.n0 + i % BN;
                 int sum = 0;
                 for (int r = 0; r < ks; ++r)
@@ -405,8 +429,18 @@ static int launch(const CUtensorMap &w_map, const CUtensorMap &a_map, const Args
                   cudaStream_t st) {
     const size_t smem = Cfg<BT>::smem(MODE == kDense ? 0 : a.E);
     auto kern = s8_gemm_kernel<BT, MODE>;
-    W4_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    W4_CUDA_TRY(launch_decode(kern, dim3(grid, 1, ks), dim3(kThreads), smem, st, ks, w_map, a_map, a));
+    {
+        static std::mutex mu;
+        static int set_dev[128] = {};
+        int dev = 0;
+        W4_CUDA_TRY(cudaGetDevice(&dev));
+        std::lock_guard<std::mutex> lk(mu);
+        if (dev >= 128 || set_dev[dev] < (int)smem) {
+            W4_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+            if (dev < 128) set_dev[dev] = (int)smem;
+        }
+    }
+    W4_CUDA_TRY(launch_decode(kern, dim3(grid, 1, ks), dim3(threads_of(MODE)), smem, st, ks, w_map, a_map, a));
     return W4_OK;
 }
 
@@ -433,7 +467,7 @@ static int map_failed() {
 int s8_gemm(const int8_t *a, const float *a_scale, const int8_t *w, const float *w_scale, const float *bias, void *c,
             int c_dtype, int M, int N, int K, cudaStream_t st) {
     using namespace s8g;
-    Args g = {a_scale, w_scale, bias, nullptr, nullptr, c, c_dtype, M, M, N, K, 1, 0, 0, (N + BN - 1) / BN};
+    Args g = {a, a_scale, w_scale, bias, nullptr, nullptr, c, c_dtype, M, M, N, K, 1, 0, 0, (N + BN - 1) / BN};
     const int BT = capacity_for(M);
     const int mt = (M + BT - 1) / BT;
     g.bt = ((M + mt - 1) / mt + 15) / 16 * 16;  // equal tiles of rows
@@ -461,7 +495,7 @@ int s8_gemm_grouped(const int8_t *a, int a_rows, const float *a_scale, const int
                     const float *bias, const int *offsets, const int *src, int E, void *c, int c_dtype, int R, int N,
                     int K, cudaStream_t st) {
     using namespace s8g;
-    Args g = {a_scale, w_scale, bias, offsets, src, c, c_dtype, R, a_rows, N, K, E, 0, 0, (N + BN - 1) / BN};
+    Args g = {a, a_scale, w_scale, bias, offsets, src, c, c_dtype, R, a_rows, N, K, E, 0, 0, (N + BN - 1) / BN};
     // The counts are on the device: capacity for about twice the average expert's rows.
     const int BT = capacity_for((int)(2L * R / E));
     g.bt = BT;
@@ -469,7 +503,7 @@ int s8_gemm_grouped(const int8_t *a, int a_rows, const float *a_scale, const int
     CUtensorMap w_map, a_map;
     if (!make_map_3d(&w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, w, K, N, E, K, (uint64_t)N * K, BK, BN,
                      CU_TENSOR_MAP_SWIZZLE_128B) ||
-        !make_map_2d(&a_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, a, K, a_rows, K, BK, src ? 1 : g.box,
+        !make_map_2d(&a_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, a, K, a_rows, K, BK, g.box,
                      CU_TENSOR_MAP_SWIZZLE_128B))
         return map_failed();
     const long most = ((long)R / g.bt + (R < E ? R : E)) * g.ntn;  // tiles at most, whatever the counts

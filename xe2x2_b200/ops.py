@@ -387,31 +387,36 @@ _FN = {None: L.W4_FN_NONE, "none": L.W4_FN_NONE, "silu_mul": L.W4_FN_SILU_MUL, "
 _FLOATS = {torch.float16: L.W4_F16, torch.bfloat16: L.W4_BF16, torch.float32: L.W4_F32}
 
 
-def _tensor(t, name, dtype, shape, dev, optional=False):
-    """Check one argument of the operators below: its dtype(s), shape, device, dense layout."""
+_S8, _I32, _F32 = frozenset({torch.int8}), frozenset({torch.int32}), frozenset({torch.float32})
+
+
+def _arg(t, name, dtypes, shape, dev, optional=False):
+    """Address of one argument of the operators below, after checking its dtype, shape, device (index
+    ``dev``) and dense layout.  These run at every call of a decode step: one test when all is well."""
     if t is None and optional:
         return None
+    if (dev >= 0 and torch.is_tensor(t) and t.dtype in dtypes and t.shape == shape and t.get_device() == dev
+            and t.is_contiguous()):
+        return t.data_ptr()
     if not torch.is_tensor(t):
         raise ValueError(f"{name} must be a tensor")
     _need_cuda(t)
-    ok = t.dtype in dtype if isinstance(dtype, (dict, tuple)) else t.dtype == dtype
-    if not ok:
-        want = ", ".join(str(d) for d in dtype) if isinstance(dtype, (dict, tuple)) else dtype
-        raise ValueError(f"{name} must be {want}, got {t.dtype}")
-    if tuple(t.shape) != tuple(shape):
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name} must be {' or '.join(sorted(str(d) for d in dtypes))}, got {t.dtype}")
+    if t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
-    if t.device != dev:
-        raise ValueError(f"{name} is on {t.device}, the first tensor on {dev}")
-    return _contig(t, name)
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, the first tensor on cuda:{dev}")
+    raise ValueError(f"{name} must be contiguous")
 
 
 def _call_on(dev, name, *args):
-    """Call an entry point on dev's current stream with dev as the current device."""
-    if dev.index == torch.cuda.current_device():
-        L.call(name, *args, _stream(dev))
+    """Call an entry point on the current stream of device index dev, with dev as the current device."""
+    if dev == torch.cuda.current_device():
+        L.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
-            L.call(name, *args, _stream(dev))
+            L.call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
 
 
 def quant_s8(x, act=None):
@@ -426,39 +431,41 @@ def quant_s8(x, act=None):
         raise ValueError(f"act must be None, 'silu_mul' or 'relu2', got {act!r}")
     if not torch.is_tensor(x) or x.dim() != 2:
         raise ValueError("x must be a 2-D tensor")
-    dev = x.device
+    dev, fn = x.get_device(), _FN[act]
     M, K = x.shape
-    _tensor(x, "x", _FLOATS, (M, K), dev)
-    if _FN[act] == L.W4_FN_SILU_MUL:
+    px = _arg(x, "x", _FLOATS, (M, K), dev)
+    if fn == L.W4_FN_SILU_MUL:
         if K % 2:
             raise ValueError("silu_mul needs x [M, 2K] (gate | up)")
         K //= 2
-    q = torch.empty((M, K), dtype=torch.int8, device=dev)
-    s = torch.empty(M, dtype=torch.float32, device=dev)
-    _call_on(dev, "w4_quant_s8", _p(x), _FLOATS[x.dtype], _FN[act], _p(q), _p(s), M, K)
+    q = x.new_empty((M, K), dtype=torch.int8)
+    s = x.new_empty(M, dtype=torch.float32)
+    _call_on(dev, "w4_quant_s8", px, _FLOATS[x.dtype], fn, q.data_ptr(), s.data_ptr(), M, K)
     return q, s
 
 
 _S8_OUT = {**_FLOATS, torch.float8_e4m3fn: L.W4_E4M3}
 
 
-def _s8_out(M, N, out_dtype, out, dev):
-    """Output tensor, row scales and scratch of an s8 GEMM.  The scratch is allocated by the call, so
-    no two streams or captured graphs share it."""
+def _s8_out(a, M, N, out_dtype, out, dev):
+    """Output tensor, row scales and scratch of an s8 GEMM on ``a``.  The scratch is allocated by the
+    call, so no two streams or captured graphs share it."""
     out_dtype = out_dtype or (out.dtype if out is not None else torch.bfloat16)
     if out_dtype not in _S8_OUT:
         raise ValueError(f"out_dtype must be f16, bf16, f32 or float8_e4m3fn, got {out_dtype}")
     if out is None:
-        out = torch.empty((M, N), dtype=out_dtype, device=dev)
+        out = a.new_empty((M, N), dtype=out_dtype)
     else:
-        _tensor(out, "out", out_dtype, (M, N), dev)
+        _arg(out, "out", (out_dtype,), (M, N), dev)
     rs = ws = None
-    need = 0
     if out_dtype == torch.float8_e4m3fn:
-        rs = torch.empty(M, dtype=torch.float32, device=dev)
-        need = L.lib().w4_s8_gemm_workspace_bytes(M, N, 16, L.W4_E4M3)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    return out, _S8_OUT[out_dtype], rs, ws, need
+        rs = a.new_empty(M, dtype=torch.float32)
+        ws = a.new_empty(L.lib().w4_s8_gemm_workspace_bytes(M, N, 16, L.W4_E4M3), dtype=torch.uint8)
+    return out, _S8_OUT[out_dtype], rs, ws
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def s8_gemm(a, a_scale, w, w_scale, bias=None, out_dtype=None, out=None):
@@ -471,16 +478,14 @@ def s8_gemm(a, a_scale, w, w_scale, bias=None, out_dtype=None, out=None):
     """
     if not torch.is_tensor(a) or a.dim() != 2 or not torch.is_tensor(w) or w.dim() != 2:
         raise ValueError("a must be [M, K] and w [N, K]")
-    dev = a.device
+    dev = a.get_device()
     (M, K), N = a.shape, w.shape[0]
-    _tensor(a, "a", torch.int8, (M, K), dev)
-    _tensor(a_scale, "a_scale", torch.float32, (M,), dev)
-    _tensor(w, "w", torch.int8, (N, K), dev)
-    _tensor(w_scale, "w_scale", torch.float32, (N,), dev)
-    _tensor(bias, "bias", torch.float32, (N,), dev, optional=True)
-    c, cdt, rs, ws, need = _s8_out(M, N, out_dtype, out, dev)
-    _call_on(dev, "w4_s8_gemm", _p(a), _p(a_scale), _p(w), _p(w_scale), _p(bias), _p(c), cdt, _p(rs), M, N, K, _p(ws),
-             need)
+    pa, pas = _arg(a, "a", _S8, (M, K), dev), _arg(a_scale, "a_scale", _F32, (M,), dev)
+    pw, pws = _arg(w, "w", _S8, (N, K), dev), _arg(w_scale, "w_scale", _F32, (N,), dev)
+    pb = _arg(bias, "bias", _F32, (N,), dev, optional=True)
+    c, cdt, rs, ws = _s8_out(a, M, N, out_dtype, out, dev)
+    _call_on(dev, "w4_s8_gemm", pa, pas, pw, pws, pb, c.data_ptr(), cdt, _ptr(rs), M, N, K, _ptr(ws),
+             0 if ws is None else ws.numel())
     return c if rs is None else (c, rs)
 
 
@@ -495,23 +500,20 @@ def s8_gemm_grouped(a, a_scale, w, w_scale, offsets, rows=None, bias=None, out_d
     """
     if not torch.is_tensor(a) or a.dim() != 2 or not torch.is_tensor(w) or w.dim() != 3:
         raise ValueError("a must be [tokens, K] and w [E, N, K]")
-    dev = a.device
-    (A, K), (E, N) = a.shape, w.shape[:2]
-    _tensor(a, "a", torch.int8, (A, K), dev)
-    _tensor(a_scale, "a_scale", torch.float32, (A,), dev)
-    _tensor(w, "w", torch.int8, (E, N, K), dev)
-    _tensor(w_scale, "w_scale", torch.float32, (E, N), dev)
-    _tensor(bias, "bias", torch.float32, (E, N), dev, optional=True)
-    _tensor(offsets, "offsets", torch.int32, (E + 1,), dev)
-    R = A
+    dev = a.get_device()
+    (A, K), (E, N, _) = a.shape, w.shape
+    pa, pas = _arg(a, "a", _S8, (A, K), dev), _arg(a_scale, "a_scale", _F32, (A,), dev)
+    pw, pws = _arg(w, "w", _S8, (E, N, K), dev), _arg(w_scale, "w_scale", _F32, (E, N), dev)
+    pb = _arg(bias, "bias", _F32, (E, N), dev, optional=True)
+    po, pr, R = _arg(offsets, "offsets", _I32, (E + 1,), dev), None, A
     if rows is not None:
         if not torch.is_tensor(rows) or rows.dim() != 1:
             raise ValueError("rows must be a 1-D tensor")
         R = rows.shape[0]
-        _tensor(rows, "rows", torch.int32, (R,), dev)
-    c, cdt, rs, ws, need = _s8_out(R, N, out_dtype, out, dev)
-    _call_on(dev, "w4_s8_gemm_grouped", _p(a), _p(a_scale), A, _p(w), _p(w_scale), _p(bias), _p(offsets), _p(rows), E,
-             _p(c), cdt, _p(rs), R, N, K, _p(ws), need)
+        pr = _arg(rows, "rows", _I32, (R,), dev)
+    c, cdt, rs, ws = _s8_out(a, R, N, out_dtype, out, dev)
+    _call_on(dev, "w4_s8_gemm_grouped", pa, pas, A, pw, pws, pb, po, pr, E, c.data_ptr(), cdt, _ptr(rs), R, N, K,
+             _ptr(ws), 0 if ws is None else ws.numel())
     return c if rs is None else (c, rs)
 
 
@@ -563,23 +565,22 @@ def moe_route(logits, top_k, bias=None, score="softmax", renormalize=True, scali
         raise ValueError(f"group_score must be 'max' or 'top2', got {group_score!r}")
     if not torch.is_tensor(logits) or logits.dim() != 2:
         raise ValueError("logits must be a 2-D tensor [tokens, experts]")
-    dev = logits.device
+    dev = logits.get_device()
     T, E = logits.shape
-    _tensor(logits, "logits", _FLOATS, (T, E), dev)
-    _tensor(bias, "bias", torch.float32, (E,), dev, optional=True)
+    pl = _arg(logits, "logits", _FLOATS, (T, E), dev)
+    pb = _arg(bias, "bias", _F32, (E,), dev, optional=True)
     top_k = int(top_k)
     if top_k < 1:
         raise ValueError(f"top_k must be at least 1, got {top_k}")
-    ids = torch.empty((T, top_k), dtype=torch.int32, device=dev)
-    weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
-    offsets = torch.empty(E + 1, dtype=torch.int32, device=dev)
-    rows = torch.empty(T * top_k, dtype=torch.int32, device=dev)
-    slots = torch.empty((T, top_k), dtype=torch.int32, device=dev)
+    i32 = torch.int32
+    ids, weights = logits.new_empty((T, top_k), dtype=i32), logits.new_empty((T, top_k), dtype=torch.float32)
+    offsets, rows = logits.new_empty(E + 1, dtype=i32), logits.new_empty(T * top_k, dtype=i32)
+    slots = logits.new_empty((T, top_k), dtype=i32)
     need = L.lib().w4_moe_route_workspace_bytes(T, E)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _call_on(dev, "w4_moe_route", _p(logits), _FLOATS[logits.dtype], _p(bias), T, E, top_k, _SCORES[score],
-             int(n_group), int(topk_group), _GROUP_SCORES[group_score], int(bool(renormalize)), float(scaling), _p(ids),
-             _p(weights), _p(offsets), _p(rows), _p(slots), _p(ws), need)
+    ws = logits.new_empty(need, dtype=torch.uint8) if need else None
+    _call_on(dev, "w4_moe_route", pl, _FLOATS[logits.dtype], pb, T, E, top_k, _SCORES[score], int(n_group),
+             int(topk_group), _GROUP_SCORES[group_score], int(bool(renormalize)), float(scaling), ids.data_ptr(),
+             weights.data_ptr(), offsets.data_ptr(), rows.data_ptr(), slots.data_ptr(), _ptr(ws), need)
     return MoERouting(ids, weights, offsets, rows, slots)
 
 
@@ -590,18 +591,17 @@ def moe_combine(y, slots, weights, add=None, out_dtype=None):
     output, the residual stream) -> [T, H] of ``out_dtype`` (default: y's)."""
     if not torch.is_tensor(y) or y.dim() != 2 or not torch.is_tensor(slots) or slots.dim() != 2:
         raise ValueError("y must be [rows, H] and slots [tokens, top_k]")
-    dev = y.device
+    dev = y.get_device()
     (rows, H), (T, k) = y.shape, slots.shape
     out_dtype = out_dtype or y.dtype
-    _tensor(y, "y", _FLOATS, (rows, H), dev)
-    _tensor(slots, "slots", torch.int32, (T, k), dev)
-    _tensor(weights, "weights", torch.float32, (T, k), dev)
+    py, ps = _arg(y, "y", _FLOATS, (rows, H), dev), _arg(slots, "slots", _I32, (T, k), dev)
+    pw = _arg(weights, "weights", _F32, (T, k), dev)
     if out_dtype not in _FLOATS:
         raise ValueError(f"out_dtype must be f16, bf16 or f32, got {out_dtype}")
-    _tensor(add, "add", out_dtype, (T, H), dev, optional=True)
-    out = torch.empty((T, H), dtype=out_dtype, device=dev)
-    _call_on(dev, "w4_moe_combine", _p(y), _FLOATS[y.dtype], rows, _p(slots), _p(weights), _p(add), _p(out),
-             _FLOATS[out_dtype], T, k, H)
+    pd = _arg(add, "add", (out_dtype,), (T, H), dev, optional=True)
+    out = y.new_empty((T, H), dtype=out_dtype)
+    _call_on(dev, "w4_moe_combine", py, _FLOATS[y.dtype], rows, ps, pw, pd, out.data_ptr(), _FLOATS[out_dtype], T, k,
+             H)
     return out
 
 
