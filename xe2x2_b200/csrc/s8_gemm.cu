@@ -15,6 +15,7 @@
 // batch of 4096 tokens x 6 experts (K 2688, N 3712, 64 experts) 1.12 ms against 0.34 ms.
 // Every wait is bounded; no copy names more than one CTA.
 #include <mutex>
+#include <type_traits>
 
 #include "tma_util.cuh"
 #include "w4_common.cuh"
@@ -41,15 +42,20 @@ struct Args {
     int c_dtype, M, a_rows, N, K, E;
     int bt, box;  // token rows of a tile (a multiple of 16), of one token copy
     int ntn;      // column tiles
+    bool wide;    // 16-bit rows of C can be stored 16 bytes at a time (N % 8 == 0, c 16-byte aligned)
 };
+
+// The epilogue's transposition buffer of a warp: 16 token pairs x 32 channels of 32 bits, rows
+// 36 words apart so that both the writes and the 16-byte reads touch every bank once.
+constexpr int TR_ROW = 36, TR_WORDS = 16 * TR_ROW;
 
 // BT token rows at most, S stages, two accumulators of BT columns.
 template <int BT> struct Cfg {
     static constexpr uint32_t T_BYTES = BT * BK, STAGE = W_BYTES + T_BYTES;
-    static constexpr int S = BT == 256 ? 4 : BT == 128 ? 6 : BT == 64 ? 9 : 12;
+    static constexpr int S = BT == 256 ? 4 : BT == 128 ? 6 : BT == 64 ? 8 : 11;
     static constexpr uint32_t TMEM_COLS = 2 * BT < 32 ? 32 : 2 * BT;
     static constexpr uint32_t BAR_OFF = S * STAGE, AS_OFF = BAR_OFF + (2 * S + 5) * 8 / 16 * 16 + 16,
-                              MISC_OFF = AS_OFF + 2 * BT * 4, TILE_OFF = MISC_OFF + 16;
+                              TR_OFF = AS_OFF + 2 * BT * 4, MISC_OFF = TR_OFF + kEpi * TR_WORDS * 4, TILE_OFF = MISC_OFF + 16;
     static constexpr uint32_t LD = BT < 32 ? BT : 32;  // columns of one TMEM read
     static constexpr int LAG = S / 2;  // stages that a gather warp's copies may be in flight
     static constexpr size_t smem(int E) { return TILE_OFF + (size_t)2 * (E + 1) * 4 + 1024; }
@@ -166,6 +172,50 @@ __device__ __forceinline__ Tile tile_of(const Args &a, int t, const int *first, 
 }
 
 __device__ __forceinline__ void store_c(const Args &a, size_t o, float v) { store_out(a.c, a.c_dtype, o, v); }
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+}
+
+// LD token columns of a warp's 32 channels, as 16-bit rows of C: pairs of tokens go through shared
+// memory word by word and come back as eight channels of one token, 16 bytes a store.
+template <int LD, typename T>
+__device__ __forceinline__ void store_rows(const Args &a, const uint32_t (&v)[LD], const float *as, float ws, float bs,
+                                           uint32_t *tr, int row, int rows, int n, int lane) {
+#pragma unroll
+    for (int i = 0; i < LD / 4; ++i) {
+        const float4 s = *reinterpret_cast<const float4 *>(as + 4 * i);
+        tr[2 * i * TR_ROW + lane] = pack2<T>(fmaf((float)(int)v[4 * i] * s.x, ws, bs),
+                                             fmaf((float)(int)v[4 * i + 1] * s.y, ws, bs));
+        tr[(2 * i + 1) * TR_ROW + lane] = pack2<T>(fmaf((float)(int)v[4 * i + 2] * s.z, ws, bs),
+                                                   fmaf((float)(int)v[4 * i + 3] * s.w, ws, bs));
+    }
+    __syncwarp();
+    const int seg = (lane & 3) * 8;  // channels n + seg .. n + seg + 7
+#pragma unroll
+    for (int h = 0; h < LD / 16; ++h) {
+        const int pair = (lane >> 2) + 8 * h;
+        const uint4 x = *reinterpret_cast<const uint4 *>(tr + pair * TR_ROW + seg);
+        const uint4 y = *reinterpret_cast<const uint4 *>(tr + pair * TR_ROW + seg + 4);
+        T *dst = static_cast<T *>(a.c) + (size_t)(row + 2 * pair) * a.N + n + seg;
+        if (n + seg < a.N && 2 * pair < rows)
+            *reinterpret_cast<uint4 *>(dst) =
+                make_uint4(__byte_perm(x.x, x.y, 0x5410), __byte_perm(x.z, x.w, 0x5410), __byte_perm(y.x, y.y, 0x5410),
+                           __byte_perm(y.z, y.w, 0x5410));
+        if (n + seg < a.N && 2 * pair + 1 < rows)
+            *reinterpret_cast<uint4 *>(dst + a.N) =
+                make_uint4(__byte_perm(x.x, x.y, 0x7632), __byte_perm(x.z, x.w, 0x7632), __byte_perm(y.x, y.y, 0x7632),
+                           __byte_perm(y.z, y.w, 0x7632));
+    }
+    __syncwarp();
+}
 
 template <int BT, int MODE>
 __global__ void __launch_bounds__(threads_of(MODE), 1)
@@ -358,6 +408,7 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
     } else {
         // ---------------- epilogue: lane quarter warp % 4 ----------------
         const int q = warp & 3, et = threadIdx.x - 64;
+        uint32_t *tr = reinterpret_cast<uint32_t *>(sm + C_::TR_OFF) + q * TR_WORDS;
         int j = 0;
         for (int t = blockIdx.x; t < ntiles; t += gridDim.x, ++j) {
             const Tile tl = tile_of<MODE>(a, t, first, off);
@@ -382,6 +433,12 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
                     int *red = reinterpret_cast<int *>(sm) + c0 * BN + 32 * q + lane;
 #pragma unroll
                     for (int i = 0; i < (int)C_::LD; ++i) red[i * BN] = (int)v[i];
+                } else if (a.wide && a.c_dtype == W4_BF16) {
+                    store_rows<C_::LD, __nv_bfloat16>(a, v, as + c0, ws, bs, tr, tl.row0 + c0, tl.rows - c0,
+                                                      tl.n0 + 32 * q, lane);
+                } else if (a.wide && a.c_dtype == W4_F16) {
+                    store_rows<C_::LD, __half>(a, v, as + c0, ws, bs, tr, tl.row0 + c0, tl.rows - c0, tl.n0 + 32 * q,
+                                               lane);
                 } else if (in) {
 #pragma unroll
                     for (int i = 0; i < (int)C_::LD; ++i)
@@ -467,7 +524,8 @@ static int map_failed() {
 int s8_gemm(const int8_t *a, const float *a_scale, const int8_t *w, const float *w_scale, const float *bias, void *c,
             int c_dtype, int M, int N, int K, cudaStream_t st) {
     using namespace s8g;
-    Args g = {a, a_scale, w_scale, bias, nullptr, nullptr, c, c_dtype, M, M, N, K, 1, 0, 0, (N + BN - 1) / BN};
+    Args g = {a, a_scale, w_scale, bias, nullptr, nullptr, c, c_dtype, M, M, N, K, 1, 0, 0, (N + BN - 1) / BN,
+              N % 8 == 0 && aligned(c, 16)};
     const int BT = capacity_for(M);
     const int mt = (M + BT - 1) / BT;
     g.bt = ((M + mt - 1) / mt + 15) / 16 * 16;  // equal tiles of rows
@@ -495,7 +553,8 @@ int s8_gemm_grouped(const int8_t *a, int a_rows, const float *a_scale, const int
                     const float *bias, const int *offsets, const int *src, int E, void *c, int c_dtype, int R, int N,
                     int K, cudaStream_t st) {
     using namespace s8g;
-    Args g = {a, a_scale, w_scale, bias, offsets, src, c, c_dtype, R, a_rows, N, K, E, 0, 0, (N + BN - 1) / BN};
+    Args g = {a, a_scale, w_scale, bias, offsets, src, c, c_dtype, R, a_rows, N, K, E, 0, 0, (N + BN - 1) / BN,
+              N % 8 == 0 && aligned(c, 16)};
     // The counts are on the device: capacity for about twice the average expert's rows.
     const int BT = capacity_for((int)(2L * R / E));
     g.bt = BT;
