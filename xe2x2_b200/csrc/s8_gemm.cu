@@ -49,10 +49,11 @@ struct Args {
 // 36 words apart so that both the writes and the 16-byte reads touch every bank once.
 constexpr int TR_ROW = 36, TR_WORDS = 16 * TR_ROW;
 
-// BT token rows at most, S stages, two accumulators of BT columns.
-template <int BT> struct Cfg {
-    static constexpr uint32_t T_BYTES = BT * BK, STAGE = W_BYTES + T_BYTES;
-    static constexpr int S = BT == 256 ? 4 : BT == 128 ? 6 : BT == 64 ? 8 : 11;
+// BT token rows at most, S stages, two accumulators of BT columns.  PAIR: two CTAs (a cluster) on one
+// tile of 256 channels; each holds its 128 channels and half of the token rows.
+template <int BT, bool PAIR> struct Cfg {
+    static constexpr uint32_t T_BYTES = (PAIR ? BT / 2 : BT) * BK, STAGE = W_BYTES + T_BYTES;
+    static constexpr int S = STAGE > 40960 ? 4 : STAGE > 28672 ? 6 : STAGE > 20480 ? 8 : 5;
     static constexpr uint32_t TMEM_COLS = 2 * BT < 32 ? 32 : 2 * BT;
     static constexpr uint32_t BAR_OFF = S * STAGE, AS_OFF = BAR_OFF + (2 * S + 5) * 8 / 16 * 16 + 16,
                               TR_OFF = AS_OFF + 2 * BT * 4, MISC_OFF = TR_OFF + kEpi * TR_WORDS * 4, TILE_OFF = MISC_OFF + 16;
@@ -62,29 +63,83 @@ template <int BT> struct Cfg {
     static_assert(TILE_OFF + 2 * (kMaxMoeExperts + 1) * 4 + 1024 <= 227 * 1024, "shared memory plan");
 };
 
+// cta_group::2 forms (PAIR) are executed by one warp of each CTA of the pair.
+template <bool PAIR>
 __device__ __forceinline__ void tmem_alloc(uint32_t *slot, uint32_t ncols) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)),
-                 "r"(ncols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if constexpr (PAIR) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)),
+                     "r"(ncols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)),
+                     "r"(ncols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
 }
+template <bool PAIR>
 __device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+    if constexpr (PAIR)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+    else
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ void tc_commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
+// The same barrier in CTA `rank` of the cluster, as a shared::cluster address; an arrival there.  The
+// default scope: what an arrival passes on is written and read by the copy engine and the tensor
+// core, ordered by their own completion mechanisms and proxy fences.  With .release.cluster /
+// .acquire.cluster on these barriers M = 8192, K = 5120, N = 17408 took 977 us instead of 519.
+__device__ __forceinline__ uint32_t bar_of(uint64_t *bar, uint32_t rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(bar)), "r"(rank));
+    return a;
 }
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+// Arrival on this CTA's barrier when the MMAs issued so far are complete (a pair's: on both SMs).
+template <bool PAIR>
+__device__ __forceinline__ void tc_commit(uint64_t *bar) {
+    if constexpr (PAIR)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                     : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                     : "memory");
+}
+template <bool PAIR>
 __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+            "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(acc)
+            : "memory");
+    else
+        asm volatile(
+            "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+            "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(acc)
+            : "memory");
+}
+// TMA loads into this CTA whose bytes count on a barrier of the pair's first CTA.
+__device__ __forceinline__ void pair_load_2d(void *dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
     asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+        "%3}], [%4];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void pair_load_3d(void *dst, const CUtensorMap *map, int x, int y, int z, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+        "%3, %4}], [%5];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
         : "memory");
 }
 // 16 bytes global -> shared, asynchronously; zeros where n is 0.
@@ -120,8 +175,8 @@ __device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr) {
            ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 // kind::i8: s32 accumulator (2 at bit 4), signed A and B (1 at bits 7 and 10), N>>3 at 17, M>>4 at 24.
-__device__ __forceinline__ uint32_t idesc_for(int n) {
-    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(BN >> 4) << 24);
+__device__ __forceinline__ uint32_t idesc_for(int n, int m) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
 __device__ __forceinline__ bool wait_s8(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
@@ -144,11 +199,14 @@ struct Tile {
     int e, row0, rows, n0;
 };
 
-__device__ __forceinline__ int round16(int v) { return (v + 15) & ~15; }
+// Token columns of a tile's MMA (M = 128: a multiple of 16; M = 256: of 32, half from each CTA).
+template <bool PAIR> __device__ __forceinline__ int mma_cols(int rows) {
+    return PAIR ? (rows + 31) & ~31 : (rows + 15) & ~15;
+}
 
 // Tile t.  Grouped: first[e] tiles before expert e, off[e] its first row; the offsets come from
 // device memory and were clamped to [0, M] and to ascending order when they were read.
-template <int MODE>
+template <int MODE, bool PAIR>
 __device__ __forceinline__ Tile tile_of(const Args &a, int t, const int *first, const int *off) {
     Tile r;
     int lo = 0, row_begin = 0, row_end = a.M, q = t;
@@ -165,7 +223,7 @@ __device__ __forceinline__ Tile tile_of(const Args &a, int t, const int *first, 
     }
     const int mt = (row_end - row_begin + a.bt - 1) / a.bt;
     r.e = lo;
-    r.n0 = q / mt * BN;
+    r.n0 = q / mt * (PAIR ? 2 * BN : BN);
     r.row0 = row_begin + q % mt * a.bt;
     r.rows = min(a.bt, row_end - r.row0);
     return r;
@@ -217,10 +275,23 @@ __device__ __forceinline__ void store_rows(const Args &a, const uint32_t (&v)[LD
     __syncwarp();
 }
 
-template <int BT, int MODE>
+// A gather warp's finished stage: every lane orders its copies into its own CTA's shared memory before
+// the tensor core's reads (the .shared::cluster form of the fence: 642 us where this takes 274, batch
+// above), then one arrival (on the first CTA's barrier, where the pair's MMAs are issued).
+template <bool PAIR>
+__device__ __forceinline__ void hand_over(uint64_t *bar, int lane) {
+    fence_proxy_async();
+    __syncwarp();
+    if (lane == 0) {
+        if constexpr (PAIR) mbar_arrive_cluster(bar_of(bar, 0));
+        else mbar_arrive(bar);
+    }
+}
+
+template <int BT, int MODE, bool PAIR>
 __global__ void __launch_bounds__(threads_of(MODE), 1)
 s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap a_map, const Args a) {
-    using C_ = Cfg<BT>;
+    using C_ = Cfg<BT, PAIR>;
     constexpr int S = C_::S;
     extern __shared__ uint8_t smem_dyn[];
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
@@ -236,18 +307,21 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
     int *off = first + a.E + 1;                                // [E + 1] its first row
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int nkb_all = (a.K + BK - 1) / BK;
-    // K split over the cluster (grid z): this CTA sums blocks [kb0, kb1) of its one tile
+    // The cluster: a pair's two CTAs along grid x, or a K split along grid z, where this CTA sums
+    // blocks [kb0, kb1) of its one tile.
+    const int rank = PAIR ? blockIdx.x & 1 : 0;
+    const int t0 = PAIR ? blockIdx.x >> 1 : blockIdx.x, tstep = PAIR ? gridDim.x >> 1 : gridDim.x;
     const int ks = gridDim.z, kr = blockIdx.z;
     const int kb0 = (int)((long)nkb_all * kr / ks), kb1 = (int)((long)nkb_all * (kr + 1) / ks);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
-            mbar_init(&full[s], MODE == kGathered ? 1 + kGather : 1);
+            mbar_init(&full[s], MODE == kGathered ? 1 + (PAIR ? 2 : 1) * kGather : 1);
             mbar_init(&empty[s], 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&acc_full[i], 1);
-            mbar_init(&acc_empty[i], kEpi);
+            mbar_init(&acc_empty[i], PAIR ? 2 * kEpi : kEpi);
         }
         mbar_init(drain, 1);
         *abort_flag = 0;
@@ -255,7 +329,7 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
         prefetch_tensormap(&w_map);
         prefetch_tensormap(&a_map);
     }
-    if (warp == 1) tmem_alloc(tmem_slot, C_::TMEM_COLS);
+    if (warp == 1) tmem_alloc<PAIR>(tmem_slot, C_::TMEM_COLS);
     grid_dep_launch();
     grid_dep_wait();
     int ntiles;
@@ -298,6 +372,7 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
     }
     tc_fence_before();
     __syncthreads();
+    if constexpr (PAIR) cluster_sync_all();  // both CTAs' barriers exist
     tc_fence_after();
     if constexpr (MODE != kDense) ntiles = first[a.E];
     const uint32_t tmem = *tmem_slot;
@@ -306,37 +381,50 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
         // ---------------- producer ----------------
         int g = 0;  // k-blocks issued (stage g % S)
         bool ok = true;
-        for (int t = blockIdx.x; t < ntiles && ok; t += gridDim.x) {
-            const Tile tl = tile_of<MODE>(a, t, first, off);
-            const int boxes = MODE == kGathered ? 0 : (round16(tl.rows) + a.box - 1) / a.box;
-            const uint32_t tx = W_BYTES + (uint32_t)(boxes * a.box) * BK;
+        for (int t = t0; t < ntiles && ok; t += tstep) {
+            const Tile tl = tile_of<MODE, PAIR>(a, t, first, off);
+            const int cols = mma_cols<PAIR>(tl.rows), mine = PAIR ? cols / 2 : cols;  // this CTA's token rows
+            const int boxes = MODE == kGathered ? 0 : (mine + a.box - 1) / a.box;
+            const uint32_t tx = (PAIR ? 2 : 1) * (W_BYTES + (uint32_t)(boxes * a.box) * BK);
             for (int kb = kb0; kb < kb1; ++kb, ++g) {
                 const int s = g % S;
-                if (g >= S && !__all_sync(0xffffffffu, wait_s8(&empty[s], (uint32_t)((g / S - 1) & 1), abort_flag))) {
-                    ok = false;
-                    break;
+                if (g >= S) {
+                    if (!__all_sync(0xffffffffu, wait_s8(&empty[s], (uint32_t)((g / S - 1) & 1), abort_flag))) {
+                        ok = false;
+                        break;
+                    }
+                    // the MMAs' commit reaches the first CTA's barrier; it tells the other one
+                    if (PAIR && rank == 0 && lane == 0) mbar_arrive_cluster(bar_of(&empty[s], 1));
                 }
                 uint8_t *w_dst = sm + s * C_::STAGE, *t_dst = w_dst + W_BYTES;
                 if (lane == 0) {
-                    mbar_arrive_expect_tx(&full[s], tx);
-                    tma_load_3d(w_dst, &w_map, kb * BK, tl.n0, tl.e, &full[s]);
-                    for (int b = 0; b < boxes; ++b)
-                        tma_load_2d(t_dst + b * a.box * BK, &a_map, kb * BK, tl.row0 + b * a.box, &full[s]);
+                    if (rank == 0) mbar_arrive_expect_tx(&full[s], tx);  // of both CTAs
+                    if constexpr (PAIR) {
+                        const uint32_t bar = bar_of(&full[s], 0);
+                        pair_load_3d(w_dst, &w_map, kb * BK, tl.n0 + rank * BN, tl.e, bar);
+                        for (int b = 0; b < boxes; ++b)
+                            pair_load_2d(t_dst + b * a.box * BK, &a_map, kb * BK,
+                                         tl.row0 + rank * mine + b * a.box, bar);
+                    } else {
+                        tma_load_3d(w_dst, &w_map, kb * BK, tl.n0, tl.e, &full[s]);
+                        for (int b = 0; b < boxes; ++b)
+                            tma_load_2d(t_dst + b * a.box * BK, &a_map, kb * BK, tl.row0 + b * a.box, &full[s]);
+                    }
                 }
             }
         }
         // after a wait that gave up, nothing of this CTA's copies may still be in flight at its end
-        if (*abort_flag)
+        if (*abort_flag && rank == 0)
             for (int i = g > S ? g - S : 0; i < g; ++i) mbar_wait_bounded(&full[i % S], (uint32_t)((i / S) & 1));
     } else if (warp == 1) {
         // ---------------- MMA issuer ----------------
-        if (lane == 0) {
+        if (lane == 0 && rank == 0) {
             const uint64_t d0 = sw128_desc(smem_u32(sm));
             int g = 0, j = 0;
             bool ok = true;
-            for (int t = blockIdx.x; t < ntiles && ok; t += gridDim.x, ++j) {
-                const Tile tl = tile_of<MODE>(a, t, first, off);
-                const uint32_t idesc = idesc_for(round16(tl.rows));
+            for (int t = t0; t < ntiles && ok; t += tstep, ++j) {
+                const Tile tl = tile_of<MODE, PAIR>(a, t, first, off);
+                const uint32_t idesc = idesc_for(mma_cols<PAIR>(tl.rows), PAIR ? 2 * BN : BN);
                 const uint32_t acc = tmem + (uint32_t)(j & 1) * BT;
                 if (j >= 2 && !wait_s8(&acc_empty[j & 1], (uint32_t)((j / 2 - 1) & 1), abort_flag)) break;
                 tc_fence_after();
@@ -350,14 +438,14 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
                     const uint64_t wd = d0 + (uint64_t)(s * (C_::STAGE >> 4)), td = wd + (W_BYTES >> 4);
                     const int steps = min(4, (a.K - kb * BK + 31) / 32);  // 32 k a step
                     for (int kk = 0; kk < steps; ++kk)
-                        mma_i8(acc, wd + 2 * kk, td + 2 * kk, idesc, kb > kb0 || kk > 0);
-                    tc_commit(&empty[s]);
+                        mma_i8<PAIR>(acc, wd + 2 * kk, td + 2 * kk, idesc, kb > kb0 || kk > 0);
+                    tc_commit<PAIR>(&empty[s]);
                 }
                 if (!ok) break;
-                tc_commit(&acc_full[j & 1]);
+                tc_commit<PAIR>(&acc_full[j & 1]);
             }
             if (*abort_flag) {  // let the MMAs in flight end before TMEM is freed
-                tc_commit(drain);
+                tc_commit<PAIR>(drain);
                 mbar_wait_bounded(drain, 0u);
             }
         }
@@ -366,18 +454,20 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
         // Thread (row r0 + 16 i, chunk c): chunk c of row r lies at c ^ (r % 8) of its 128-byte line.
         // A stage is handed over LAG stages after its copies were issued: each thread waits for its
         // own, orders them before the tensor core's reads (proxy fence), and lane 0 arrives.
-        constexpr int LAG = C_::LAG, ROWS = kGather * 32 / 8, NR = (BT + ROWS - 1) / ROWS;
+        constexpr int LAG = C_::LAG, ROWS = kGather * 32 / 8, NR = ((PAIR ? BT / 2 : BT) + ROWS - 1) / ROWS;
         const int gt = threadIdx.x - 32 * (2 + kEpi), r0 = gt >> 3, c = gt & 7;
         const uint32_t line = (uint32_t)(r0 * BK + ((c ^ (r0 & 7)) << 4));  // ROWS is a multiple of 8
         int g = 0;
         bool ok = true;
-        for (int t = blockIdx.x; t < ntiles && ok; t += gridDim.x) {
-            const Tile tl = tile_of<MODE>(a, t, first, off);
+        for (int t = t0; t < ntiles && ok; t += tstep) {
+            const Tile tl = tile_of<MODE, PAIR>(a, t, first, off);
+            const int begin = rank * (mma_cols<PAIR>(tl.rows) / 2);  // this CTA's first row, and how many
+            const int mine = PAIR && rank == 0 ? min(tl.rows, mma_cols<PAIR>(tl.rows) / 2) : tl.rows - begin;
             const int8_t *row[NR];
 #pragma unroll
             for (int i = 0; i < NR; ++i) {
                 const int r = r0 + i * ROWS;
-                const int src = r < tl.rows ? a.src[tl.row0 + r] : 0;
+                const int src = r < mine ? a.src[tl.row0 + begin + r] : 0;
                 row[i] = a.a + (size_t)(src >= 0 && src < a.a_rows ? src : 0) * a.K;  // else scaled by 0
             }
             for (int kb = kb0; kb < kb1; ++kb, ++g) {
@@ -390,40 +480,36 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
                 const uint32_t n = x < a.K ? 16u : 0u, dst = smem_u32(sm + s * C_::STAGE + W_BYTES) + line;
 #pragma unroll
                 for (int i = 0; i < NR; ++i)
-                    if (r0 + i * ROWS < tl.rows) cp_async16_zfill(dst + i * ROWS * BK, row[i] + (n ? x : 0), n);
+                    if (r0 + i * ROWS < mine) cp_async16_zfill(dst + i * ROWS * BK, row[i] + (n ? x : 0), n);
                 cp_async_commit();
                 if (g >= LAG) {
                     cp_async_wait<LAG>();
-                    fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&full[(g - LAG) % S]);
+                    hand_over<PAIR>(&full[(g - LAG) % S], lane);
                 }
             }
         }
         cp_async_wait<0>();
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0)
-            for (int i = g > LAG ? g - LAG : 0; i < g; ++i) mbar_arrive(&full[i % S]);
+        for (int i = g > LAG ? g - LAG : 0; i < g; ++i) hand_over<PAIR>(&full[i % S], lane);
     } else {
         // ---------------- epilogue: lane quarter warp % 4 ----------------
         const int q = warp & 3, et = threadIdx.x - 64;
         uint32_t *tr = reinterpret_cast<uint32_t *>(sm + C_::TR_OFF) + q * TR_WORDS;
         int j = 0;
-        for (int t = blockIdx.x; t < ntiles; t += gridDim.x, ++j) {
-            const Tile tl = tile_of<MODE>(a, t, first, off);
+        for (int t = t0; t < ntiles; t += tstep, ++j) {
+            const Tile tl = tile_of<MODE, PAIR>(a, t, first, off);
             float *as = as_sh + (j & 1) * BT;
             for (int i = et; i < tl.rows; i += kEpi * 32) {
                 int r = tl.row0 + i;
                 if constexpr (MODE == kGathered) r = a.src[r];
                 as[i] = MODE != kGathered || (r >= 0 && r < a.a_rows) ? a.a_scale[r] : 0.f;
             }
-            const int n = tl.n0 + 32 * q + lane;
+            const int n0 = tl.n0 + rank * BN, n = n0 + 32 * q + lane;
             const bool in = n < a.N;
             const float ws = in ? a.w_scale[(size_t)tl.e * a.N + n] : 0.f;
             const float bs = in && a.bias ? a.bias[(size_t)tl.e * a.N + n] : 0.f;
             asm volatile("bar.sync 1, %0;" ::"r"(kEpi * 32) : "memory");  // as[] is complete
             if (!__all_sync(0xffffffffu, wait_s8(&acc_full[j & 1], (uint32_t)((j / 2) & 1), abort_flag))) break;
+            if (PAIR && rank == 0 && et == 0) mbar_arrive_cluster(bar_of(&acc_full[j & 1], 1));
             tc_fence_after();
             const uint32_t acc = tmem + (uint32_t)(j & 1) * BT + ((uint32_t)(32 * q) << 16);
             for (int c0 = 0; c0 < tl.rows; c0 += C_::LD) {
@@ -435,9 +521,9 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
                     for (int i = 0; i < (int)C_::LD; ++i) red[i * BN] = (int)v[i];
                 } else if (a.wide && a.c_dtype == W4_BF16) {
                     store_rows<C_::LD, __nv_bfloat16>(a, v, as + c0, ws, bs, tr, tl.row0 + c0, tl.rows - c0,
-                                                      tl.n0 + 32 * q, lane);
+                                                      n0 + 32 * q, lane);
                 } else if (a.wide && a.c_dtype == W4_F16) {
-                    store_rows<C_::LD, __half>(a, v, as + c0, ws, bs, tr, tl.row0 + c0, tl.rows - c0, tl.n0 + 32 * q,
+                    store_rows<C_::LD, __half>(a, v, as + c0, ws, bs, tr, tl.row0 + c0, tl.rows - c0, n0 + 32 * q,
                                                lane);
                 } else if (in) {
 #pragma unroll
@@ -449,21 +535,26 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&acc_empty[j & 1]);
+            if (lane == 0) {
+                if constexpr (PAIR) mbar_arrive_cluster(bar_of(&acc_empty[j & 1], 0));
+                else mbar_arrive(&acc_empty[j & 1]);
+            }
         }
     }
     tc_fence_before();
     __syncthreads();
+    if constexpr (PAIR) cluster_sync_all();  // both CTAs are done with TMEM and each other's barriers
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem, C_::TMEM_COLS);
+        tmem_dealloc<PAIR>(tmem, C_::TMEM_COLS);
     }
+    if constexpr (PAIR) cluster_sync_all();
     if (ks > 1) {
         // Every CTA of the cluster holds its part of one tile's sums (s32: the order does not
         // matter) where its stages were; each finishes an equal share of the tile.
         cluster_sync_all();
         if ((int)blockIdx.x < ntiles) {
-            const Tile tl = tile_of<MODE>(a, blockIdx.x, first, off);
+            const Tile tl = tile_of<MODE, PAIR>(a, blockIdx.x, first, off);
             const int total = tl.rows * BN;
             const int i1 = (int)((long)total * (kr + 1) / ks);
             for (int i = (int)((long)total * kr / ks) + threadIdx.x; i < i1; i += blockDim.x) {
@@ -481,11 +572,11 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
     }
 }
 
-template <int BT, int MODE>
+template <int BT, int MODE, bool PAIR = false>
 static int launch(const CUtensorMap &w_map, const CUtensorMap &a_map, const Args &a, int grid, int ks,
                   cudaStream_t st) {
-    const size_t smem = Cfg<BT>::smem(MODE == kDense ? 0 : a.E);
-    auto kern = s8_gemm_kernel<BT, MODE>;
+    const size_t smem = Cfg<BT, PAIR>::smem(MODE == kDense ? 0 : a.E);
+    auto kern = s8_gemm_kernel<BT, MODE, PAIR>;
     {
         static std::mutex mu;
         static int set_dev[128] = {};
@@ -497,7 +588,8 @@ static int launch(const CUtensorMap &w_map, const CUtensorMap &a_map, const Args
             if (dev < 128) set_dev[dev] = (int)smem;
         }
     }
-    W4_CUDA_TRY(launch_decode(kern, dim3(grid, 1, ks), dim3(threads_of(MODE)), smem, st, ks, w_map, a_map, a));
+    W4_CUDA_TRY(launch_cluster(kern, dim3(PAIR ? 2 * grid : grid, 1, ks), dim3(threads_of(MODE)), smem, st,
+                               dim3(PAIR ? 2 : 1, 1, ks), w_map, a_map, a));
     return W4_OK;
 }
 
@@ -508,7 +600,8 @@ static int launch_bt(int BT, const CUtensorMap &w_map, const CUtensorMap &a_map,
         case 16: return launch<16, MODE>(w_map, a_map, a, grid, ks, st);
         case 64: return launch<64, MODE>(w_map, a_map, a, grid, ks, st);
         case 128: return launch<128, MODE>(w_map, a_map, a, grid, ks, st);
-        default: return launch<256, MODE>(w_map, a_map, a, grid, ks, st);
+        case 256: return launch<256, MODE>(w_map, a_map, a, grid, ks, st);
+        default: return launch<256, MODE, true>(w_map, a_map, a, grid, ks, st);
     }
 }
 
@@ -521,15 +614,21 @@ static int map_failed() {
 
 }  // namespace s8g
 
+constexpr int kPairTile = 512;  // launch_bt's name for the 256-row tile of a CTA pair
+
 int s8_gemm(const int8_t *a, const float *a_scale, const int8_t *w, const float *w_scale, const float *bias, void *c,
             int c_dtype, int M, int N, int K, cudaStream_t st) {
     using namespace s8g;
-    Args g = {a, a_scale, w_scale, bias, nullptr, nullptr, c, c_dtype, M, M, N, K, 1, 0, 0, (N + BN - 1) / BN,
-              N % 8 == 0 && aligned(c, 16)};
-    const int BT = capacity_for(M);
+    const int nsm = num_sms(), nkb = (K + BK - 1) / BK;
+    int BT = capacity_for(M);
     const int mt = (M + BT - 1) / BT;
-    g.bt = ((M + mt - 1) / mt + 15) / 16 * 16;  // equal tiles of rows
-    g.box = g.bt;
+    bool pair = BT == 256;
+    Args g = {a, a_scale, w_scale, bias, nullptr, nullptr, c, c_dtype, M, M, N, K, 1, 0, 0, 0,
+              N % 8 == 0 && aligned(c, 16)};
+    const int step = pair ? 32 : 16;
+    g.bt = ((M + mt - 1) / mt + step - 1) / step * step;  // equal tiles of rows
+    g.box = pair ? g.bt / 2 : g.bt;
+    g.ntn = pair ? (N + 2 * BN - 1) / (2 * BN) : (N + BN - 1) / BN;
     CUtensorMap w_map, a_map;
     if (!make_map_3d(&w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, w, K, N, 1, K, (uint64_t)N * K, BK, BN,
                      CU_TENSOR_MAP_SWIZZLE_128B) ||
@@ -537,10 +636,10 @@ int s8_gemm(const int8_t *a, const float *a_scale, const int8_t *w, const float 
         return map_failed();
     const long tiles = (long)((M + g.bt - 1) / g.bt) * g.ntn;
     W4_REQUIRE(tiles < (1L << 30), W4_ERR_UNSUPPORTED, "s8 GEMM: %ld tiles", tiles);
+    if (pair) return launch_bt<kDense>(kPairTile, w_map, a_map, g, (int)(tiles < nsm / 2 ? tiles : nsm / 2), 1, st);
     // Few tiles: a cluster splits K, at least four blocks to a CTA.
     int ks = 1;
-    const int nsm = num_sms(), nkb = (K + BK - 1) / BK;
-    if (2 * tiles <= nsm && BT <= 128) {
+    if (2 * tiles <= nsm) {
         ks = (int)(nsm / tiles);
         ks = ks > 8 ? 8 : ks;
         ks = ks > nkb / 4 ? nkb / 4 : ks;
@@ -553,23 +652,22 @@ int s8_gemm_grouped(const int8_t *a, int a_rows, const float *a_scale, const int
                     const float *bias, const int *offsets, const int *src, int E, void *c, int c_dtype, int R, int N,
                     int K, cudaStream_t st) {
     using namespace s8g;
-    Args g = {a, a_scale, w_scale, bias, offsets, src, c, c_dtype, R, a_rows, N, K, E, 0, 0, (N + BN - 1) / BN,
-              N % 8 == 0 && aligned(c, 16)};
     // The counts are on the device: capacity for about twice the average expert's rows.
     const int BT = capacity_for((int)(2L * R / E));
-    g.bt = BT;
-    g.box = BT < 32 ? BT : 32;
+    const bool pair = BT == 256;
+    Args g = {a, a_scale, w_scale, bias, offsets, src, c, c_dtype, R, a_rows, N, K, E, BT, BT < 32 ? BT : 32, 0,
+              N % 8 == 0 && aligned(c, 16)};
+    g.ntn = pair ? (N + 2 * BN - 1) / (2 * BN) : (N + BN - 1) / BN;
     CUtensorMap w_map, a_map;
     if (!make_map_3d(&w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, w, K, N, E, K, (uint64_t)N * K, BK, BN,
                      CU_TENSOR_MAP_SWIZZLE_128B) ||
-        !make_map_2d(&a_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, a, K, a_rows, K, BK, g.box,
-                     CU_TENSOR_MAP_SWIZZLE_128B))
+        !make_map_2d(&a_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, a, K, a_rows, K, BK, g.box, CU_TENSOR_MAP_SWIZZLE_128B))
         return map_failed();
     const long most = ((long)R / g.bt + (R < E ? R : E)) * g.ntn;  // tiles at most, whatever the counts
     W4_REQUIRE(most < (1L << 30), W4_ERR_UNSUPPORTED, "s8 GEMM: %ld tiles", most);
-    const int grid = (int)(most < num_sms() ? most : num_sms());
-    return src ? launch_bt<kGathered>(BT, w_map, a_map, g, grid, 1, st)
-               : launch_bt<kGrouped>(BT, w_map, a_map, g, grid, 1, st);
+    const int slots = pair ? num_sms() / 2 : num_sms(), grid = (int)(most < slots ? most : slots);
+    return src ? launch_bt<kGathered>(pair ? kPairTile : BT, w_map, a_map, g, grid, 1, st)
+               : launch_bt<kGrouped>(pair ? kPairTile : BT, w_map, a_map, g, grid, 1, st);
 }
 
 int take_s8_wait_status() {

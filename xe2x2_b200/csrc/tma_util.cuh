@@ -162,13 +162,13 @@ inline PFN_cuTensorMapEncodeTiled encode_fn() {
     return fn;
 }
 
-// Launch of a decode kernel, with programmatic stream serialisation unless the
-// overlap mode is W4_OVERLAP_OFF: the kernel may then start while the previous
-// kernel on the stream drains, and orders itself behind it with grid_dep_wait().
-// cluster_z > 1: thread-block clusters of (1, 1, cluster_z) CTAs along grid z.
+// Launch with programmatic stream serialisation unless the overlap mode is
+// W4_OVERLAP_OFF: the kernel may then start while the previous kernel on the
+// stream drains, and orders itself behind it with grid_dep_wait().  cluster:
+// the thread-block cluster's shape (1, 1, 1 for none).
 template <typename... KArgs, typename... Args>
-inline cudaError_t launch_decode(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
-                                 unsigned cluster_z, Args &&...args) {
+inline cudaError_t launch_cluster(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
+                                  dim3 cluster, Args &&...args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
@@ -181,16 +181,23 @@ inline cudaError_t launch_decode(void (*kern)(KArgs...), dim3 grid, dim3 block, 
         at[n].val.programmaticStreamSerializationAllowed = 1;
         ++n;
     }
-    if (cluster_z > 1) {
+    if (cluster.x * cluster.y * cluster.z > 1) {
         at[n].id = cudaLaunchAttributeClusterDimension;
-        at[n].val.clusterDim.x = 1;
-        at[n].val.clusterDim.y = 1;
-        at[n].val.clusterDim.z = cluster_z;
+        at[n].val.clusterDim.x = cluster.x;
+        at[n].val.clusterDim.y = cluster.y;
+        at[n].val.clusterDim.z = cluster.z;
         ++n;
     }
     cfg.attrs = at;
     cfg.numAttrs = n;
     return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+}
+
+// The same for a decode kernel, whose clusters are (1, 1, cluster_z) CTAs along grid z.
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_decode(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
+                                 unsigned cluster_z, Args &&...args) {
+    return launch_cluster(kern, grid, block, smem, st, dim3(1, 1, cluster_z), std::forward<Args>(args)...);
 }
 
 // 3-D tiled map of [d2][d1][d0] elements (d0 innermost; byte strides s1 of d1 and s2 of d2), box
