@@ -102,6 +102,15 @@ __device__ __forceinline__ uint32_t bar_of(uint64_t *bar, uint32_t rank) {
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
+__device__ __forceinline__ int4 ld_cluster_v4(const void *p, uint32_t rank) {
+    uint32_t a;
+    int4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(a));
+    return v;
+}
 // Arrival on this CTA's barrier when the MMAs issued so far are complete (a pair's: on both SMs).
 template <bool PAIR>
 __device__ __forceinline__ void tc_commit(uint64_t *bar) {
@@ -279,11 +288,11 @@ __device__ __forceinline__ void store_rows(const Args &a, const uint32_t (&v)[LD
 // the tensor core's reads (the .shared::cluster form of the fence: 642 us where this takes 274, batch
 // above), then one arrival (on the first CTA's barrier, where the pair's MMAs are issued).
 template <bool PAIR>
-__device__ __forceinline__ void hand_over(uint64_t *bar, int lane) {
+__device__ __forceinline__ void hand_over(uint64_t *bar, uint32_t lead, int lane) {
     fence_proxy_async();
     __syncwarp();
     if (lane == 0) {
-        if constexpr (PAIR) mbar_arrive_cluster(bar_of(bar, 0));
+        if constexpr (PAIR) mbar_arrive_cluster(bar_of(bar, lead));
         else mbar_arrive(bar);
     }
 }
@@ -307,9 +316,10 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
     int *off = first + a.E + 1;                                // [E + 1] its first row
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int nkb_all = (a.K + BK - 1) / BK;
-    // The cluster: a pair's two CTAs along grid x, or a K split along grid z, where this CTA sums
+    // The cluster: a pair's two CTAs along x, and along z a K split, where this CTA (or pair) sums
     // blocks [kb0, kb1) of its one tile.
     const int rank = PAIR ? blockIdx.x & 1 : 0;
+    const uint32_t lead = 2 * blockIdx.z;  // the pair's first CTA
     const int t0 = PAIR ? blockIdx.x >> 1 : blockIdx.x, tstep = PAIR ? gridDim.x >> 1 : gridDim.x;
     const int ks = gridDim.z, kr = blockIdx.z;
     const int kb0 = (int)((long)nkb_all * kr / ks), kb1 = (int)((long)nkb_all * (kr + 1) / ks);
@@ -379,7 +389,8 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
 
     if (warp == 0) {
         // ---------------- producer ----------------
-        int g = 0;  // k-blocks issued (stage g % S)
+        int g = 0, s = 0;  // k-blocks issued, their stage
+        uint32_t phase = 1;  // a fresh barrier's "previous" phase counts as complete
         bool ok = true;
         for (int t = t0; t < ntiles && ok; t += tstep) {
             const Tile tl = tile_of<MODE, PAIR>(a, t, first, off);
@@ -387,20 +398,17 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
             const int boxes = MODE == kGathered ? 0 : (mine + a.box - 1) / a.box;
             const uint32_t tx = (PAIR ? 2 : 1) * (W_BYTES + (uint32_t)(boxes * a.box) * BK);
             for (int kb = kb0; kb < kb1; ++kb, ++g) {
-                const int s = g % S;
-                if (g >= S) {
-                    if (!__all_sync(0xffffffffu, wait_s8(&empty[s], (uint32_t)((g / S - 1) & 1), abort_flag))) {
-                        ok = false;
-                        break;
-                    }
-                    // the MMAs' commit reaches the first CTA's barrier; it tells the other one
-                    if (PAIR && rank == 0 && lane == 0) mbar_arrive_cluster(bar_of(&empty[s], 1));
+                if (!__all_sync(0xffffffffu, wait_s8(&empty[s], phase, abort_flag))) {
+                    ok = false;
+                    break;
                 }
                 uint8_t *w_dst = sm + s * C_::STAGE, *t_dst = w_dst + W_BYTES;
                 if (lane == 0) {
+                    // the MMAs' commit reaches the first CTA's barrier; it tells the other one
+                    if (PAIR && rank == 0 && g >= S) mbar_arrive_cluster(bar_of(&empty[s], lead + 1));
                     if (rank == 0) mbar_arrive_expect_tx(&full[s], tx);  // of both CTAs
                     if constexpr (PAIR) {
-                        const uint32_t bar = bar_of(&full[s], 0);
+                        const uint32_t bar = bar_of(&full[s], lead);
                         pair_load_3d(w_dst, &w_map, kb * BK, tl.n0 + rank * BN, tl.e, bar);
                         for (int b = 0; b < boxes; ++b)
                             pair_load_2d(t_dst + b * a.box * BK, &a_map, kb * BK,
@@ -411,6 +419,11 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
                             tma_load_2d(t_dst + b * a.box * BK, &a_map, kb * BK, tl.row0 + b * a.box, &full[s]);
                     }
                 }
+                __syncwarp();
+                if (++s == S) {
+                    s = 0;
+                    phase ^= 1;
+                }
             }
         }
         // after a wait that gave up, nothing of this CTA's copies may still be in flight at its end
@@ -418,33 +431,43 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
             for (int i = g > S ? g - S : 0; i < g; ++i) mbar_wait_bounded(&full[i % S], (uint32_t)((i / S) & 1));
     } else if (warp == 1) {
         // ---------------- MMA issuer ----------------
-        if (lane == 0 && rank == 0) {
+        // The whole warp runs the loop and one lane issues, so that every operand is warp-uniform:
+        // inside a one-lane branch each MMA cost 105 cycles of register moves, 780 a stage with the
+        // wait, whatever its N (128 k: 512 cycles of tensor work at N = 256, 32 at N = 16).
+        if (rank == 0) {
             const uint64_t d0 = sw128_desc(smem_u32(sm));
-            int g = 0, j = 0;
+            int s = 0, j = 0;
+            uint32_t phase = 0;
             bool ok = true;
             for (int t = t0; t < ntiles && ok; t += tstep, ++j) {
                 const Tile tl = tile_of<MODE, PAIR>(a, t, first, off);
                 const uint32_t idesc = idesc_for(mma_cols<PAIR>(tl.rows), PAIR ? 2 * BN : BN);
                 const uint32_t acc = tmem + (uint32_t)(j & 1) * BT;
-                if (j >= 2 && !wait_s8(&acc_empty[j & 1], (uint32_t)((j / 2 - 1) & 1), abort_flag)) break;
+                if (j >= 2 && !__all_sync(0xffffffffu, wait_s8(&acc_empty[j & 1], (uint32_t)((j / 2 - 1) & 1), abort_flag)))
+                    break;
                 tc_fence_after();
-                for (int kb = kb0; kb < kb1; ++kb, ++g) {
-                    const int s = g % S;
-                    if (!wait_s8(&full[s], (uint32_t)((g / S) & 1), abort_flag)) {
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    if (!__all_sync(0xffffffffu, wait_s8(&full[s], phase, abort_flag))) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
                     const uint64_t wd = d0 + (uint64_t)(s * (C_::STAGE >> 4)), td = wd + (W_BYTES >> 4);
-                    const int steps = min(4, (a.K - kb * BK + 31) / 32);  // 32 k a step
-                    for (int kk = 0; kk < steps; ++kk)
-                        mma_i8<PAIR>(acc, wd + 2 * kk, td + 2 * kk, idesc, kb > kb0 || kk > 0);
-                    tc_commit<PAIR>(&empty[s]);
+                    if (lane == 0) {
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk)  // 32 k a step; zeros behind K
+                            mma_i8<PAIR>(acc, wd + 2 * kk, td + 2 * kk, idesc, kb > kb0 || kk > 0);
+                        tc_commit<PAIR>(&empty[s]);
+                        if (kb == kb1 - 1) tc_commit<PAIR>(&acc_full[j & 1]);
+                    }
+                    __syncwarp();
+                    if (++s == S) {
+                        s = 0;
+                        phase ^= 1;
+                    }
                 }
-                if (!ok) break;
-                tc_commit<PAIR>(&acc_full[j & 1]);
             }
-            if (*abort_flag) {  // let the MMAs in flight end before TMEM is freed
+            if (*abort_flag && lane == 0) {  // let the MMAs in flight end before TMEM is freed
                 tc_commit<PAIR>(drain);
                 mbar_wait_bounded(drain, 0u);
             }
@@ -484,12 +507,12 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
                 cp_async_commit();
                 if (g >= LAG) {
                     cp_async_wait<LAG>();
-                    hand_over<PAIR>(&full[(g - LAG) % S], lane);
+                    hand_over<PAIR>(&full[(g - LAG) % S], lead, lane);
                 }
             }
         }
         cp_async_wait<0>();
-        for (int i = g > LAG ? g - LAG : 0; i < g; ++i) hand_over<PAIR>(&full[i % S], lane);
+        for (int i = g > LAG ? g - LAG : 0; i < g; ++i) hand_over<PAIR>(&full[i % S], lead, lane);
     } else {
         // ---------------- epilogue: lane quarter warp % 4 ----------------
         const int q = warp & 3, et = threadIdx.x - 64;
@@ -509,7 +532,7 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
             const float bs = in && a.bias ? a.bias[(size_t)tl.e * a.N + n] : 0.f;
             asm volatile("bar.sync 1, %0;" ::"r"(kEpi * 32) : "memory");  // as[] is complete
             if (!__all_sync(0xffffffffu, wait_s8(&acc_full[j & 1], (uint32_t)((j / 2) & 1), abort_flag))) break;
-            if (PAIR && rank == 0 && et == 0) mbar_arrive_cluster(bar_of(&acc_full[j & 1], 1));
+            if (PAIR && rank == 0 && et == 0) mbar_arrive_cluster(bar_of(&acc_full[j & 1], lead + 1));
             tc_fence_after();
             const uint32_t acc = tmem + (uint32_t)(j & 1) * BT + ((uint32_t)(32 * q) << 16);
             for (int c0 = 0; c0 < tl.rows; c0 += C_::LD) {
@@ -536,7 +559,7 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
-                if constexpr (PAIR) mbar_arrive_cluster(bar_of(&acc_empty[j & 1], 0));
+                if constexpr (PAIR) mbar_arrive_cluster(bar_of(&acc_empty[j & 1], lead));
                 else mbar_arrive(&acc_empty[j & 1]);
             }
         }
@@ -550,22 +573,54 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
     }
     if constexpr (PAIR) cluster_sync_all();
     if (ks > 1) {
-        // Every CTA of the cluster holds its part of one tile's sums (s32: the order does not
-        // matter) where its stages were; each finishes an equal share of the tile.
+        // The CTAs along z hold their parts of one tile's sums (s32: the order does not matter) where
+        // their stages were; each finishes an equal share of the rows, a warp a row, four channels a
+        // lane, four rows in flight.
         cluster_sync_all();
-        if ((int)blockIdx.x < ntiles) {
-            const Tile tl = tile_of<MODE, PAIR>(a, blockIdx.x, first, off);
-            const int total = tl.rows * BN;
-            const int i1 = (int)((long)total * (kr + 1) / ks);
-            for (int i = (int)((long)total * kr / ks) + threadIdx.x; i < i1; i += blockDim.x) {
-                const int row = i / BN, n = tl.n0 + i % BN;
-                int sum = 0;
-                for (int r = 0; r < ks; ++r)
-                    sum += __float_as_int(ld_cluster_f32(reinterpret_cast<const float *>(sm) + i, (uint32_t)r));
-                if (n < a.N)
-                    store_c(a, (size_t)(tl.row0 + row) * a.N + n,
-                            fmaf((float)sum * as_sh[row], a.w_scale[(size_t)tl.e * a.N + n],
-                                 a.bias ? a.bias[(size_t)tl.e * a.N + n] : 0.f));
+        if (t0 < ntiles) {
+            const Tile tl = tile_of<MODE, PAIR>(a, t0, first, off);
+            const int n = tl.n0 + rank * BN + 4 * lane, warps = blockDim.x >> 5;
+            float ws[4], bs[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                ws[u] = n + u < a.N ? a.w_scale[(size_t)tl.e * a.N + n + u] : 0.f;
+                bs[u] = n + u < a.N && a.bias ? a.bias[(size_t)tl.e * a.N + n + u] : 0.f;
+            }
+            const int r1 = tl.rows * (kr + 1) / ks;
+            for (int r0 = tl.rows * kr / ks + warp; r0 < r1; r0 += 4 * warps) {
+                int v[4][4] = {};
+#pragma unroll 4
+                for (int z = 0; z < ks; ++z)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int row = min(r0 + i * warps, r1 - 1);
+                        const int4 p = ld_cluster_v4(sm + (row * BN + 4 * lane) * 4, PAIR ? 2 * z + rank : z);
+                        v[i][0] += p.x;
+                        v[i][1] += p.y;
+                        v[i][2] += p.z;
+                        v[i][3] += p.w;
+                    }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = r0 + i * warps;
+                    if (row >= r1 || n >= a.N) continue;
+                    const float as = as_sh[row];
+                    float y[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) y[u] = fmaf((float)v[i][u] * as, ws[u], bs[u]);
+                    const size_t o = (size_t)(tl.row0 + row) * a.N + n;
+                    if (a.wide && a.c_dtype == W4_BF16) {
+                        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.c) + o) =
+                            make_uint2(pack2<__nv_bfloat16>(y[0], y[1]), pack2<__nv_bfloat16>(y[2], y[3]));
+                    } else if (a.wide && a.c_dtype == W4_F16) {
+                        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.c) + o) =
+                            make_uint2(pack2<__half>(y[0], y[1]), pack2<__half>(y[2], y[3]));
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < 4; ++u)
+                            if (n + u < a.N) store_c(a, o + u, y[u]);
+                    }
+                }
             }
         }
         cluster_sync_all();  // nobody leaves while its sums are read
@@ -594,18 +649,57 @@ static int launch(const CUtensorMap &w_map, const CUtensorMap &a_map, const Args
 }
 
 template <int MODE>
-static int launch_bt(int BT, const CUtensorMap &w_map, const CUtensorMap &a_map, const Args &a, int grid, int ks,
-                     cudaStream_t st) {
+static int launch_bt(int BT, bool pair, const CUtensorMap &w_map, const CUtensorMap &a_map, const Args &a, int grid,
+                     int ks, cudaStream_t st) {
+    if (pair) return launch<256, MODE, true>(w_map, a_map, a, grid, ks, st);
     switch (BT) {
         case 16: return launch<16, MODE>(w_map, a_map, a, grid, ks, st);
         case 64: return launch<64, MODE>(w_map, a_map, a, grid, ks, st);
         case 128: return launch<128, MODE>(w_map, a_map, a, grid, ks, st);
-        case 256: return launch<256, MODE>(w_map, a_map, a, grid, ks, st);
-        default: return launch<256, MODE, true>(w_map, a_map, a, grid, ks, st);
+        default: return launch<256, MODE>(w_map, a_map, a, grid, ks, st);
     }
 }
 
-static int capacity_for(int rows) { return rows <= 16 ? 16 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256; }
+// Tile of a call: capacity BT (with PAIR for two CTAs), bt token rows used of it, K split ks.
+struct Plan {
+    int BT, bt, ks, ntn;
+    bool pair;
+    long tiles;
+};
+
+// The plan with the least estimated cycles.  A k-block of 128 takes 2 bt tensor cycles, or longer to
+// arrive at 64 bytes a cycle and SM (128 channels and bt rows; a pair's CTA has half of the rows);
+// tiles go in waves over the SMs; a K split (a cluster of at most 8 CTAs, four k-blocks each at
+// least, one tile a cluster) costs an exchange; and nothing is faster than memory.
+static Plan plan_for(int M, int N, int K) {
+    const int nsm = num_sms(), nkb = (K + BK - 1) / BK;
+    Plan best = {};
+    double least = 0;
+    const double memory = ((double)N * K + (double)M * K + 2.0 * M * N) / 3500;  // cycles at 6.5 TB/s
+    for (int c = 0; c < 5; ++c) {
+        Plan p;
+        p.BT = c == 0 ? 16 : c == 1 ? 64 : c == 2 ? 128 : 256;
+        p.pair = c == 4;
+        if (c > 0 && c < 4 && M <= p.BT / 4) continue;  // far wider than the batch
+        const int step = p.pair ? 32 : 16, mt = (M + p.BT - 1) / p.BT;
+        p.bt = ((M + mt - 1) / mt + step - 1) / step * step;  // equal tiles of rows
+        p.ntn = p.pair ? (N + 2 * BN - 1) / (2 * BN) : (N + BN - 1) / BN;
+        p.tiles = (long)((M + p.bt - 1) / p.bt) * p.ntn;
+        const int slots = p.pair ? nsm / 2 : nsm;
+        const double per_kb = p.pair ? (256 + p.bt > 2 * p.bt ? 256 + p.bt : 2 * p.bt) : 256 + 2 * p.bt;
+        for (p.ks = 1; p.ks <= (p.pair ? 4 : 8); ++p.ks) {
+            if (p.ks > 1 && (p.tiles * p.ks > slots || nkb / p.ks < 4)) break;
+            const double waves = (double)((p.tiles * p.ks + slots - 1) / slots);
+            double t = waves * ((nkb + p.ks - 1) / p.ks) * per_kb;
+            t = (t > memory ? t : memory) + 10.0 * p.bt + (p.ks > 1 ? 2500 + 12.0 * p.bt / p.ks : 0);
+            if (least == 0 || t < least) {
+                least = t;
+                best = p;
+            }
+        }
+    }
+    return best;
+}
 
 static int map_failed() {
     set_error("s8 GEMM: the tensor map of an operand was refused (shape or alignment)");
@@ -614,38 +708,20 @@ static int map_failed() {
 
 }  // namespace s8g
 
-constexpr int kPairTile = 512;  // launch_bt's name for the 256-row tile of a CTA pair
-
 int s8_gemm(const int8_t *a, const float *a_scale, const int8_t *w, const float *w_scale, const float *bias, void *c,
             int c_dtype, int M, int N, int K, cudaStream_t st) {
     using namespace s8g;
-    const int nsm = num_sms(), nkb = (K + BK - 1) / BK;
-    int BT = capacity_for(M);
-    const int mt = (M + BT - 1) / BT;
-    bool pair = BT == 256;
-    Args g = {a, a_scale, w_scale, bias, nullptr, nullptr, c, c_dtype, M, M, N, K, 1, 0, 0, 0,
-              N % 8 == 0 && aligned(c, 16)};
-    const int step = pair ? 32 : 16;
-    g.bt = ((M + mt - 1) / mt + step - 1) / step * step;  // equal tiles of rows
-    g.box = pair ? g.bt / 2 : g.bt;
-    g.ntn = pair ? (N + 2 * BN - 1) / (2 * BN) : (N + BN - 1) / BN;
+    const Plan p = plan_for(M, N, K);
+    const Args g = {a, a_scale, w_scale, bias, nullptr, nullptr, c, c_dtype, M, M, N, K, 1, p.bt,
+                    p.pair ? p.bt / 2 : p.bt, p.ntn, N % 8 == 0 && aligned(c, 16)};
     CUtensorMap w_map, a_map;
     if (!make_map_3d(&w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, w, K, N, 1, K, (uint64_t)N * K, BK, BN,
                      CU_TENSOR_MAP_SWIZZLE_128B) ||
         !make_map_2d(&a_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, a, K, M, K, BK, g.box, CU_TENSOR_MAP_SWIZZLE_128B))
         return map_failed();
-    const long tiles = (long)((M + g.bt - 1) / g.bt) * g.ntn;
-    W4_REQUIRE(tiles < (1L << 30), W4_ERR_UNSUPPORTED, "s8 GEMM: %ld tiles", tiles);
-    if (pair) return launch_bt<kDense>(kPairTile, w_map, a_map, g, (int)(tiles < nsm / 2 ? tiles : nsm / 2), 1, st);
-    // Few tiles: a cluster splits K, at least four blocks to a CTA.
-    int ks = 1;
-    if (2 * tiles <= nsm) {
-        ks = (int)(nsm / tiles);
-        ks = ks > 8 ? 8 : ks;
-        ks = ks > nkb / 4 ? nkb / 4 : ks;
-        ks = ks < 1 ? 1 : ks;
-    }
-    return launch_bt<kDense>(BT, w_map, a_map, g, (int)(tiles < nsm ? tiles : nsm), ks, st);
+    W4_REQUIRE(p.tiles < (1L << 30), W4_ERR_UNSUPPORTED, "s8 GEMM: %ld tiles", p.tiles);
+    const int slots = p.pair ? num_sms() / 2 : num_sms();
+    return launch_bt<kDense>(p.BT, p.pair, w_map, a_map, g, (int)(p.tiles < slots ? p.tiles : slots), p.ks, st);
 }
 
 int s8_gemm_grouped(const int8_t *a, int a_rows, const float *a_scale, const int8_t *w, const float *w_scale,
@@ -653,11 +729,11 @@ int s8_gemm_grouped(const int8_t *a, int a_rows, const float *a_scale, const int
                     int K, cudaStream_t st) {
     using namespace s8g;
     // The counts are on the device: capacity for about twice the average expert's rows.
-    const int BT = capacity_for((int)(2L * R / E));
-    const bool pair = BT == 256;
-    Args g = {a, a_scale, w_scale, bias, offsets, src, c, c_dtype, R, a_rows, N, K, E, BT, BT < 32 ? BT : 32, 0,
-              N % 8 == 0 && aligned(c, 16)};
-    g.ntn = pair ? (N + 2 * BN - 1) / (2 * BN) : (N + BN - 1) / BN;
+    const long rows = 2L * R / E;
+    const int BT = rows <= 16 ? 16 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+    const bool pair = BT == 256 && N > BN;
+    const Args g = {a, a_scale, w_scale, bias, offsets, src, c, c_dtype, R, a_rows, N, K, E, BT, BT < 32 ? BT : 32,
+                    pair ? (N + 2 * BN - 1) / (2 * BN) : (N + BN - 1) / BN, N % 8 == 0 && aligned(c, 16)};
     CUtensorMap w_map, a_map;
     if (!make_map_3d(&w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, w, K, N, E, K, (uint64_t)N * K, BK, BN,
                      CU_TENSOR_MAP_SWIZZLE_128B) ||
@@ -666,8 +742,8 @@ int s8_gemm_grouped(const int8_t *a, int a_rows, const float *a_scale, const int
     const long most = ((long)R / g.bt + (R < E ? R : E)) * g.ntn;  // tiles at most, whatever the counts
     W4_REQUIRE(most < (1L << 30), W4_ERR_UNSUPPORTED, "s8 GEMM: %ld tiles", most);
     const int slots = pair ? num_sms() / 2 : num_sms(), grid = (int)(most < slots ? most : slots);
-    return src ? launch_bt<kGathered>(pair ? kPairTile : BT, w_map, a_map, g, grid, 1, st)
-               : launch_bt<kGrouped>(pair ? kPairTile : BT, w_map, a_map, g, grid, 1, st);
+    return src ? launch_bt<kGathered>(BT, pair, w_map, a_map, g, grid, 1, st)
+               : launch_bt<kGrouped>(BT, pair, w_map, a_map, g, grid, 1, st);
 }
 
 int take_s8_wait_status() {
