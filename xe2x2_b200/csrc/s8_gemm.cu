@@ -188,9 +188,13 @@ __device__ __forceinline__ uint32_t idesc_for(int n, int m) {
     return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
+// Bounded wait.  The clock is read only after some tries: reading it costs about as much as a stage
+// of the decode GEMM takes.
 __device__ __forceinline__ bool wait_s8(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
     const uint32_t b = smem_u32(bar);
-    if (mbar_try_wait(b, parity)) return true;
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+        if (mbar_try_wait(b, parity)) return true;
     const unsigned long long t0 = global_ns();
     while (!mbar_try_wait(b, parity)) {
         if (*abort_flag) return false;
@@ -201,6 +205,14 @@ __device__ __forceinline__ bool wait_s8(uint64_t *bar, uint32_t parity, volatile
         }
     }
     return true;
+}
+
+// One lane of a converged warp, in the form from which the compiler knows that it is one: a copy or an
+// MMA inside needs no loop over the lanes that might execute it.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(one));
+    return one != 0;
 }
 
 // A tile: rows [row0, row0 + rows) of C (and of A, unless gathered), channels from n0 of expert e.
@@ -403,7 +415,7 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
                     break;
                 }
                 uint8_t *w_dst = sm + s * C_::STAGE, *t_dst = w_dst + W_BYTES;
-                if (lane == 0) {
+                if (elect_one()) {
                     // the MMAs' commit reaches the first CTA's barrier; it tells the other one
                     if (PAIR && rank == 0 && g >= S) mbar_arrive_cluster(bar_of(&empty[s], lead + 1));
                     if (rank == 0) mbar_arrive_expect_tx(&full[s], tx);  // of both CTAs
@@ -453,7 +465,7 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
                     }
                     tc_fence_after();
                     const uint64_t wd = d0 + (uint64_t)(s * (C_::STAGE >> 4)), td = wd + (W_BYTES >> 4);
-                    if (lane == 0) {
+                    if (elect_one()) {
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)  // 32 k a step; zeros behind K
                             mma_i8<PAIR>(acc, wd + 2 * kk, td + 2 * kk, idesc, kb > kb0 || kk > 0);
