@@ -399,9 +399,13 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
     if constexpr (MODE != kDense) ntiles = first[a.E];
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == 0) {
+    // Warps 0 and 1 leave their loops to one lane (elect_one): a wait by all 32 lanes costs 190 cycles
+    // on a barrier that is complete already, and inside a branch on the lane number each MMA cost
+    // another 105 of register moves; a stage took 780 cycles whatever its N, where the tensor work of
+    // 128 k is 512 at N = 256 and 32 at N = 16.
+    if (warp == 0 && elect_one()) {
         // ---------------- producer ----------------
-        int g = 0, s = 0;  // k-blocks issued, their stage
+        int g = 0, s = 0;    // k-blocks issued, their stage
         uint32_t phase = 1;  // a fresh barrier's "previous" phase counts as complete
         bool ok = true;
         for (int t = t0; t < ntiles && ok; t += tstep) {
@@ -410,28 +414,24 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
             const int boxes = MODE == kGathered ? 0 : (mine + a.box - 1) / a.box;
             const uint32_t tx = (PAIR ? 2 : 1) * (W_BYTES + (uint32_t)(boxes * a.box) * BK);
             for (int kb = kb0; kb < kb1; ++kb, ++g) {
-                if (!__all_sync(0xffffffffu, wait_s8(&empty[s], phase, abort_flag))) {
+                if (!wait_s8(&empty[s], phase, abort_flag)) {
                     ok = false;
                     break;
                 }
                 uint8_t *w_dst = sm + s * C_::STAGE, *t_dst = w_dst + W_BYTES;
-                if (elect_one()) {
-                    // the MMAs' commit reaches the first CTA's barrier; it tells the other one
-                    if (PAIR && rank == 0 && g >= S) mbar_arrive_cluster(bar_of(&empty[s], lead + 1));
-                    if (rank == 0) mbar_arrive_expect_tx(&full[s], tx);  // of both CTAs
-                    if constexpr (PAIR) {
-                        const uint32_t bar = bar_of(&full[s], lead);
-                        pair_load_3d(w_dst, &w_map, kb * BK, tl.n0 + rank * BN, tl.e, bar);
-                        for (int b = 0; b < boxes; ++b)
-                            pair_load_2d(t_dst + b * a.box * BK, &a_map, kb * BK,
-                                         tl.row0 + rank * mine + b * a.box, bar);
-                    } else {
-                        tma_load_3d(w_dst, &w_map, kb * BK, tl.n0, tl.e, &full[s]);
-                        for (int b = 0; b < boxes; ++b)
-                            tma_load_2d(t_dst + b * a.box * BK, &a_map, kb * BK, tl.row0 + b * a.box, &full[s]);
-                    }
+                // the MMAs' commit reaches the first CTA's barrier; it tells the other one
+                if (PAIR && rank == 0 && g >= S) mbar_arrive_cluster(bar_of(&empty[s], lead + 1));
+                if (rank == 0) mbar_arrive_expect_tx(&full[s], tx);  // of both CTAs
+                if constexpr (PAIR) {
+                    const uint32_t bar = bar_of(&full[s], lead);
+                    pair_load_3d(w_dst, &w_map, kb * BK, tl.n0 + rank * BN, tl.e, bar);
+                    for (int b = 0; b < boxes; ++b)
+                        pair_load_2d(t_dst + b * a.box * BK, &a_map, kb * BK, tl.row0 + rank * mine + b * a.box, bar);
+                } else {
+                    tma_load_3d(w_dst, &w_map, kb * BK, tl.n0, tl.e, &full[s]);
+                    for (int b = 0; b < boxes; ++b)
+                        tma_load_2d(t_dst + b * a.box * BK, &a_map, kb * BK, tl.row0 + b * a.box, &full[s]);
                 }
-                __syncwarp();
                 if (++s == S) {
                     s = 0;
                     phase ^= 1;
@@ -441,49 +441,42 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
         // after a wait that gave up, nothing of this CTA's copies may still be in flight at its end
         if (*abort_flag && rank == 0)
             for (int i = g > S ? g - S : 0; i < g; ++i) mbar_wait_bounded(&full[i % S], (uint32_t)((i / S) & 1));
-    } else if (warp == 1) {
+    } else if (warp == 1 && rank == 0 && elect_one()) {
         // ---------------- MMA issuer ----------------
-        // The whole warp runs the loop and one lane issues, so that every operand is warp-uniform:
-        // inside a one-lane branch each MMA cost 105 cycles of register moves, 780 a stage with the
-        // wait, whatever its N (128 k: 512 cycles of tensor work at N = 256, 32 at N = 16).
-        if (rank == 0) {
-            const uint64_t d0 = sw128_desc(smem_u32(sm));
-            int s = 0, j = 0;
-            uint32_t phase = 0;
-            bool ok = true;
-            for (int t = t0; t < ntiles && ok; t += tstep, ++j) {
-                const Tile tl = tile_of<MODE, PAIR>(a, t, first, off);
-                const uint32_t idesc = idesc_for(mma_cols<PAIR>(tl.rows), PAIR ? 2 * BN : BN);
-                const uint32_t acc = tmem + (uint32_t)(j & 1) * BT;
-                if (j >= 2 && !__all_sync(0xffffffffu, wait_s8(&acc_empty[j & 1], (uint32_t)((j / 2 - 1) & 1), abort_flag)))
+        const uint64_t d0 = sw128_desc(smem_u32(sm));
+        int s = 0, j = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int t = t0; t < ntiles && ok; t += tstep, ++j) {
+            const Tile tl = tile_of<MODE, PAIR>(a, t, first, off);
+            const uint32_t idesc = idesc_for(mma_cols<PAIR>(tl.rows), PAIR ? 2 * BN : BN);
+            const uint32_t acc = tmem + (uint32_t)(j & 1) * BT;
+            if (j >= 2 && !wait_s8(&acc_empty[j & 1], (uint32_t)((j / 2 - 1) & 1), abort_flag)) break;
+            tc_fence_after();
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!wait_s8(&full[s], phase, abort_flag)) {
+                    ok = false;
                     break;
+                }
                 tc_fence_after();
-                for (int kb = kb0; kb < kb1; ++kb) {
-                    if (!__all_sync(0xffffffffu, wait_s8(&full[s], phase, abort_flag))) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint64_t wd = d0 + (uint64_t)(s * (C_::STAGE >> 4)), td = wd + (W_BYTES >> 4);
-                    if (elect_one()) {
+                const uint64_t wd = d0 + (uint64_t)(s * (C_::STAGE >> 4)), td = wd + (W_BYTES >> 4);
 #pragma unroll
-                        for (int kk = 0; kk < 4; ++kk)  // 32 k a step; zeros behind K
-                            mma_i8<PAIR>(acc, wd + 2 * kk, td + 2 * kk, idesc, kb > kb0 || kk > 0);
-                        tc_commit<PAIR>(&empty[s]);
-                        if (kb == kb1 - 1) tc_commit<PAIR>(&acc_full[j & 1]);
-                    }
-                    __syncwarp();
-                    if (++s == S) {
-                        s = 0;
-                        phase ^= 1;
-                    }
+                for (int kk = 0; kk < 4; ++kk)  // 32 k a step; zeros behind K
+                    mma_i8<PAIR>(acc, wd + 2 * kk, td + 2 * kk, idesc, kb > kb0 || kk > 0);
+                tc_commit<PAIR>(&empty[s]);
+                if (++s == S) {
+                    s = 0;
+                    phase ^= 1;
                 }
             }
-            if (*abort_flag && lane == 0) {  // let the MMAs in flight end before TMEM is freed
-                tc_commit<PAIR>(drain);
-                mbar_wait_bounded(drain, 0u);
-            }
+            if (ok) tc_commit<PAIR>(&acc_full[j & 1]);
         }
+        if (*abort_flag) {  // let the MMAs in flight end before TMEM is freed
+            tc_commit<PAIR>(drain);
+            mbar_wait_bounded(drain, 0u);
+        }
+    } else if (warp < 2) {
+        // the other lanes wait at the end
     } else if (MODE == kGathered && warp >= 2 + kEpi) {
         // ---------------- gather: token rows through the index, 16 bytes a thread and copy ----------------
         // Thread (row r0 + 16 i, chunk c): chunk c of row r lies at c ^ (r % 8) of its 128-byte line.
