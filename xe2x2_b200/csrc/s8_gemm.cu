@@ -58,7 +58,6 @@ template <int BT, bool PAIR> struct Cfg {
     static constexpr uint32_t BAR_OFF = S * STAGE, AS_OFF = BAR_OFF + (2 * S + 5) * 8 / 16 * 16 + 16,
                               TR_OFF = AS_OFF + 2 * BT * 4, MISC_OFF = TR_OFF + kEpi * TR_WORDS * 4, TILE_OFF = MISC_OFF + 16;
     static constexpr uint32_t LD = BT < 32 ? BT : 32;  // columns of one TMEM read
-    static constexpr int LAG = S / 2;  // stages that a gather warp's copies may be in flight
     static constexpr size_t smem(int E) { return TILE_OFF + (size_t)2 * (E + 1) * 4 + 1024; }
     static_assert(TILE_OFF + 2 * (kMaxMoeExperts + 1) * 4 + 1024 <= 227 * 1024, "shared memory plan");
 };
@@ -338,7 +337,7 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
-            mbar_init(&full[s], MODE == kGathered ? 1 + (PAIR ? 2 : 1) * kGather : 1);
+            mbar_init(&full[s], MODE == kGathered ? (PAIR ? 3 : 2) : 1);
             mbar_init(&empty[s], 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -478,46 +477,45 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
     } else if (warp < 2) {
         // the other lanes wait at the end
     } else if (MODE == kGathered && warp >= 2 + kEpi) {
-        // ---------------- gather: token rows through the index, 16 bytes a thread and copy ----------------
-        // Thread (row r0 + 16 i, chunk c): chunk c of row r lies at c ^ (r % 8) of its 128-byte line.
-        // A stage is handed over LAG stages after its copies were issued: each thread waits for its
-        // own, orders them before the tensor core's reads (proxy fence), and lane 0 arrives.
-        constexpr int LAG = C_::LAG, ROWS = kGather * 32 / 8, NR = ((PAIR ? BT / 2 : BT) + ROWS - 1) / ROWS;
-        const int gt = threadIdx.x - 32 * (2 + kEpi), r0 = gt >> 3, c = gt & 7;
-        const uint32_t line = (uint32_t)(r0 * BK + ((c ^ (r0 & 7)) << 4));  // ROWS is a multiple of 8
+        // ---------------- gather: token rows through the index, 16 bytes a lane and copy ----------------
+        // The warps take the stages in turn.  Lane (r, c) of four rows a copy: chunk c of row r lies at
+        // c ^ (r % 8) of its 128-byte line.  Row numbers are spread over the lanes, 32 a register.
+        constexpr int ROWS = PAIR ? BT / 2 : BT;
+        const int r0 = lane >> 3, c = lane & 7;
         int g = 0;
         bool ok = true;
         for (int t = t0; t < ntiles && ok; t += tstep) {
             const Tile tl = tile_of<MODE, PAIR>(a, t, first, off);
-            const int begin = rank * (mma_cols<PAIR>(tl.rows) / 2);  // this CTA's first row, and how many
-            const int mine = PAIR && rank == 0 ? min(tl.rows, mma_cols<PAIR>(tl.rows) / 2) : tl.rows - begin;
-            const int8_t *row[NR];
+            const int half = mma_cols<PAIR>(tl.rows) / 2, begin = rank * half;  // this CTA's first row
+            const int mine = PAIR && rank == 0 ? min(tl.rows, half) : tl.rows - begin;
+            int src[(ROWS + 31) / 32];
 #pragma unroll
-            for (int i = 0; i < NR; ++i) {
-                const int r = r0 + i * ROWS;
-                const int src = r < mine ? a.src[tl.row0 + begin + r] : 0;
-                row[i] = a.a + (size_t)(src >= 0 && src < a.a_rows ? src : 0) * a.K;  // else scaled by 0
+            for (int i = 0; i < (ROWS + 31) / 32; ++i) {
+                const int r = 32 * i + lane;
+                src[i] = r < mine ? a.src[tl.row0 + begin + r] : 0;
+                if (src[i] < 0 || src[i] >= a.a_rows) src[i] = 0;  // scaled by 0
             }
             for (int kb = kb0; kb < kb1; ++kb, ++g) {
+                if (g % kGather != warp - (2 + kEpi)) continue;
                 const int s = g % S;
                 if (g >= S && !__all_sync(0xffffffffu, wait_s8(&empty[s], (uint32_t)((g / S - 1) & 1), abort_flag))) {
                     ok = false;
                     break;
                 }
                 const int x = kb * BK + c * 16;
-                const uint32_t n = x < a.K ? 16u : 0u, dst = smem_u32(sm + s * C_::STAGE + W_BYTES) + line;
+                const uint32_t n = x < a.K ? 16u : 0u, line = smem_u32(sm + s * C_::STAGE + W_BYTES) + r0 * BK;
+                const int8_t *col = a.a + (n ? x : 0);
 #pragma unroll
-                for (int i = 0; i < NR; ++i)
-                    if (r0 + i * ROWS < mine) cp_async16_zfill(dst + i * ROWS * BK, row[i] + (n ? x : 0), n);
-                cp_async_commit();
-                if (g >= LAG) {
-                    cp_async_wait<LAG>();
-                    hand_over<PAIR>(&full[(g - LAG) % S], lead, lane);
+                for (int i = 0; i < ROWS / 4; ++i) {
+                    const int r = 4 * i + r0;
+                    const int row = __shfl_sync(0xffffffffu, src[i / 8], r & 31);
+                    if (r < mine) cp_async16_zfill(line + i * 4 * BK + ((c ^ (r & 7)) << 4), col + (size_t)row * a.K, n);
                 }
+                cp_async_commit();
+                cp_async_wait<0>();
+                hand_over<PAIR>(&full[s], lead, lane);
             }
         }
-        cp_async_wait<0>();
-        for (int i = g > LAG ? g - LAG : 0; i < g; ++i) hand_over<PAIR>(&full[i % S], lead, lane);
     } else {
         // ---------------- epilogue: lane quarter warp % 4 ----------------
         const int q = warp & 3, et = threadIdx.x - 64;
