@@ -9,7 +9,7 @@
 // one kernel serves every batch: N is 16 for a decode step and 256 for a prompt, and the MMA's N
 // follows the rows that a tile has.  Both operands are K-major 128-byte lines, 128-byte swizzle,
 // fetched by TMA; K is padded with zeros by the copy itself.  Warp 0 produces, warp 1 issues the
-// MMAs, warps 2-5 read the sums out of TMEM (two accumulators: one fills while the other is read),
+// MMAs, warps 2 to 5 or 9 read the sums out of TMEM (two accumulators: one fills while the other is read),
 // scale and store.  Token rows that are gathered through an index come by 16-byte cp.async from
 // four more warps: TMA's tile::gather4 (four rows a copy) took 55 to 75 cycles a copy, which made a
 // batch of 4096 tokens x 6 experts (K 2688, N 3712, 64 experts) 1.12 ms against 0.34 ms.
@@ -28,11 +28,14 @@ static __device__ unsigned int g_s8_timeout;  // a bounded wait expired (sticky 
 namespace s8g {
 
 constexpr int BN = 128, BK = 128;  // output channels and bytes of K in a stage
-constexpr int kEpi = 4, kGather = 4;  // epilogue and gather warps (2-5 and 6-9)
+constexpr int kGather = 4;  // gather warps
+// Epilogue warps (from warp 2 on): two to a lane quarter for the widest tile.  16 bytes a store hardly
+// need the second one (M = 24,576, K = 2688, N = 3712, bf16: 175 and 181 us), f32 and odd N do (262 -> 215).
+constexpr int epi_warps(int bt) { return bt == 256 ? 8 : 4; }
 constexpr uint32_t W_BYTES = BN * BK;
 
 enum Mode { kDense = 0, kGrouped = 1, kGathered = 2 };
-constexpr int threads_of(int mode) { return 32 * (2 + kEpi + (mode == kGathered ? kGather : 0)); }
+constexpr int threads_of(int bt, int mode) { return 32 * (2 + epi_warps(bt) + (mode == kGathered ? kGather : 0)); }
 
 struct Args {
     const int8_t *a;  // gathered rows only (TMA has its map)
@@ -52,11 +55,13 @@ constexpr int TR_ROW = 36, TR_WORDS = 16 * TR_ROW;
 // BT token rows at most, S stages, two accumulators of BT columns.  PAIR: two CTAs (a cluster) on one
 // tile of 256 channels; each holds its 128 channels and half of the token rows.
 template <int BT, bool PAIR> struct Cfg {
+    static constexpr int EPI = epi_warps(BT);
     static constexpr uint32_t T_BYTES = (PAIR ? BT / 2 : BT) * BK, STAGE = W_BYTES + T_BYTES;
     static constexpr int S = STAGE > 40960 ? 4 : STAGE > 28672 ? 6 : STAGE > 20480 ? 8 : 5;
     static constexpr uint32_t TMEM_COLS = 2 * BT < 32 ? 32 : 2 * BT;
     static constexpr uint32_t BAR_OFF = S * STAGE, AS_OFF = BAR_OFF + (2 * S + 5) * 8 / 16 * 16 + 16,
-                              TR_OFF = AS_OFF + 2 * BT * 4, MISC_OFF = TR_OFF + kEpi * TR_WORDS * 4, TILE_OFF = MISC_OFF + 16;
+                              TR_OFF = AS_OFF + 2 * BT * 4, MISC_OFF = TR_OFF + EPI * TR_WORDS * 4,
+                              TILE_OFF = MISC_OFF + 16;
     static constexpr uint32_t LD = BT < 32 ? BT : 32;  // columns of one TMEM read
     static constexpr size_t smem(int E) { return TILE_OFF + (size_t)2 * (E + 1) * 4 + 1024; }
     static_assert(TILE_OFF + 2 * (kMaxMoeExperts + 1) * 4 + 1024 <= 227 * 1024, "shared memory plan");
@@ -308,11 +313,28 @@ __device__ __forceinline__ void hand_over(uint64_t *bar, uint32_t lead, int lane
     }
 }
 
+// The same column by column, for rows that cannot be stored in 16 bytes (f32, odd N): a warp's 32
+// channels of one token are one store.
+template <int LD, typename T>
+__device__ __forceinline__ void store_cols(const Args &a, const uint32_t (&v)[LD], const float *as, float ws, float bs,
+                                           int row, int rows, int n) {
+    T *dst = static_cast<T *>(a.c) + (size_t)row * a.N + n;
+#pragma unroll
+    for (int i = 0; i < LD; ++i) {
+        if (i < rows) {
+            const float y = fmaf((float)(int)v[i] * as[i], ws, bs);
+            if constexpr (sizeof(T) == 4) *dst = y;
+            else *dst = Conv<T>::from_f(y);
+        }
+        dst += a.N;
+    }
+}
+
 template <int BT, int MODE, bool PAIR>
-__global__ void __launch_bounds__(threads_of(MODE), 1)
+__global__ void __launch_bounds__(threads_of(BT, MODE), 1)
 s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap a_map, const Args a) {
     using C_ = Cfg<BT, PAIR>;
-    constexpr int S = C_::S;
+    constexpr int S = C_::S, EPI = C_::EPI;
     extern __shared__ uint8_t smem_dyn[];
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
     uint64_t *full = reinterpret_cast<uint64_t *>(sm + C_::BAR_OFF);
@@ -342,7 +364,7 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&acc_full[i], 1);
-            mbar_init(&acc_empty[i], PAIR ? 2 * kEpi : kEpi);
+            mbar_init(&acc_empty[i], PAIR ? 2 * EPI : EPI);
         }
         mbar_init(drain, 1);
         *abort_flag = 0;
@@ -476,7 +498,7 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
         }
     } else if (warp < 2) {
         // the other lanes wait at the end
-    } else if (MODE == kGathered && warp >= 2 + kEpi) {
+    } else if (MODE == kGathered && warp >= 2 + EPI) {
         // ---------------- gather: token rows through the index, 16 bytes a lane and copy ----------------
         // The warps take the stages in turn.  Lane (r, c) of four rows a copy: chunk c of row r lies at
         // c ^ (r % 8) of its 128-byte line.  Row numbers are spread over the lanes, 32 a register.
@@ -496,7 +518,7 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
                 if (src[i] < 0 || src[i] >= a.a_rows) src[i] = 0;  // scaled by 0
             }
             for (int kb = kb0; kb < kb1; ++kb, ++g) {
-                if (g % kGather != warp - (2 + kEpi)) continue;
+                if (g % kGather != warp - (2 + EPI)) continue;
                 const int s = g % S;
                 if (g >= S && !__all_sync(0xffffffffu, wait_s8(&empty[s], (uint32_t)((g / S - 1) & 1), abort_flag))) {
                     ok = false;
@@ -518,13 +540,14 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
         }
     } else {
         // ---------------- epilogue: lane quarter warp % 4 ----------------
-        const int q = warp & 3, et = threadIdx.x - 64;
-        uint32_t *tr = reinterpret_cast<uint32_t *>(sm + C_::TR_OFF) + q * TR_WORDS;
+        const int q = warp & 3, ew = warp - 2;
+        uint32_t *tr = reinterpret_cast<uint32_t *>(sm + C_::TR_OFF) + ew * TR_WORDS;
+        bool ok = true;
         int j = 0;
         for (int t = t0; t < ntiles; t += tstep, ++j) {
             const Tile tl = tile_of<MODE, PAIR>(a, t, first, off);
             float *as = as_sh + (j & 1) * BT;
-            for (int i = et; i < tl.rows; i += kEpi * 32) {
+            for (int i = threadIdx.x - 64; i < tl.rows; i += EPI * 32) {
                 int r = tl.row0 + i;
                 if constexpr (MODE == kGathered) r = a.src[r];
                 as[i] = MODE != kGathered || (r >= 0 && r < a.a_rows) ? a.a_scale[r] : 0.f;
@@ -533,12 +556,15 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
             const bool in = n < a.N;
             const float ws = in ? a.w_scale[(size_t)tl.e * a.N + n] : 0.f;
             const float bs = in && a.bias ? a.bias[(size_t)tl.e * a.N + n] : 0.f;
-            asm volatile("bar.sync 1, %0;" ::"r"(kEpi * 32) : "memory");  // as[] is complete
-            if (!__all_sync(0xffffffffu, wait_s8(&acc_full[j & 1], (uint32_t)((j / 2) & 1), abort_flag))) break;
-            if (PAIR && rank == 0 && et == 0) mbar_arrive_cluster(bar_of(&acc_full[j & 1], lead + 1));
+            // as[] is complete (and the other one read).  A warp whose wait gave up still comes here for
+            // every tile, so that the others are never left waiting.
+            asm volatile("bar.sync 1, %0;" ::"r"(EPI * 32) : "memory");
+            ok = ok && __all_sync(0xffffffffu, wait_s8(&acc_full[j & 1], (uint32_t)((j / 2) & 1), abort_flag));
+            if (!ok) continue;
+            if (PAIR && rank == 0 && ew == 0 && lane == 0) mbar_arrive_cluster(bar_of(&acc_full[j & 1], lead + 1));
             tc_fence_after();
             const uint32_t acc = tmem + (uint32_t)(j & 1) * BT + ((uint32_t)(32 * q) << 16);
-            for (int c0 = 0; c0 < tl.rows; c0 += C_::LD) {
+            for (int c0 = ew / 4 * C_::LD; c0 < tl.rows; c0 += EPI / 4 * C_::LD) {
                 uint32_t v[C_::LD];
                 tmem_ld<C_::LD>(acc + c0, v);
                 if (ks > 1) {  // raw sums, summed over the cluster below
@@ -552,11 +578,11 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
                     store_rows<C_::LD, __half>(a, v, as + c0, ws, bs, tr, tl.row0 + c0, tl.rows - c0, n0 + 32 * q,
                                                lane);
                 } else if (in) {
-#pragma unroll
-                    for (int i = 0; i < (int)C_::LD; ++i)
-                        if (c0 + i < tl.rows)
-                            store_c(a, (size_t)(tl.row0 + c0 + i) * a.N + n,
-                                    fmaf((float)(int)v[i] * as[c0 + i], ws, bs));
+                    if (a.c_dtype == W4_F32)
+                        store_cols<C_::LD, float>(a, v, as + c0, ws, bs, tl.row0 + c0, tl.rows - c0, n);
+                    else if (a.c_dtype == W4_BF16)
+                        store_cols<C_::LD, __nv_bfloat16>(a, v, as + c0, ws, bs, tl.row0 + c0, tl.rows - c0, n);
+                    else store_cols<C_::LD, __half>(a, v, as + c0, ws, bs, tl.row0 + c0, tl.rows - c0, n);
                 }
             }
             tc_fence_before();
@@ -646,7 +672,7 @@ static int launch(const CUtensorMap &w_map, const CUtensorMap &a_map, const Args
             if (dev < 128) set_dev[dev] = (int)smem;
         }
     }
-    W4_CUDA_TRY(launch_cluster(kern, dim3(PAIR ? 2 * grid : grid, 1, ks), dim3(threads_of(MODE)), smem, st,
+    W4_CUDA_TRY(launch_cluster(kern, dim3(PAIR ? 2 * grid : grid, 1, ks), dim3(threads_of(BT, MODE)), smem, st,
                                dim3(PAIR ? 2 : 1, 1, ks), w_map, a_map, a));
     return W4_OK;
 }
