@@ -9,9 +9,9 @@ from xe2x2_b200 import ops
 pytestmark = pytest.mark.gpu
 
 DTYPES = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
-# relative error of y: expf is within 1 ulp (2^-23), the sum, the quotient and the product round
-# once each (2^-24); the scale's division rounds once more
-Y_REL = {None: 0.0, "relu2": 2.0 ** -24, "silu_mul": 5 * 2.0 ** -24}
+# relative error of y: expf is within 1 ulp (2^-23), the sum and the product round once each (2^-24),
+# the quotient is within 2 ulp (2^-22, __fdividef); the scale's division rounds once more
+Y_REL = {None: 0.0, "relu2": 2.0 ** -24, "silu_mul": 2.0 ** -23 + 2 * 2.0 ** -24 + 2.0 ** -22}
 
 
 def _y64(x, act):
@@ -86,6 +86,33 @@ def test_rows_with_nan_or_infinity(cuda):
     assert not q[1:4].any()
     q0, s0 = ops.quant_s8(x[[0, 4]].contiguous())
     assert torch.equal(q[[0, 4]], q0) and torch.equal(s[[0, 4]], s0)
+
+
+@pytest.mark.parametrize("size", [1e-45, 1e-41, 1e-38, 3e-36, 1e-29, 1e-20, 3e38])
+def test_tiny_and_huge_rows_equal_f32_arithmetic(cuda, size):
+    """Scales down to the smallest subnormals (a scale that rounds to 0 becomes 1) and near the largest."""
+    g = torch.Generator(device=cuda).manual_seed(3)
+    x = (torch.rand(8, 512, generator=g, device=cuda) * 2 - 1) * size
+    x[:, ::7] *= 0.5
+    q, s = ops.quant_s8(x)
+    xf = np_(x)
+    amax = np.abs(xf).max(1)
+    want = (amax / np.float32(127)).astype(np.float32)
+    want = np.where(want > 0, want, np.float32(1)).astype(np.float32)
+    assert np.array_equal(np_(s), want)
+    ref = np.clip(np.rint((xf / want[:, None]).astype(np.float32)), -127, 127)
+    assert np.array_equal(np_(q).astype(np.float32), ref)
+
+
+def test_halves_of_the_maximum_round_to_even(cuda):
+    """x = max / 2 is a tie in real arithmetic (63.5): decided as y / s rounds in f32."""
+    for dt in DTYPES.values():
+        a = torch.linspace(0.5, 8.0, 64, device=cuda).to(dt)
+        x = (a[:, None].float() * torch.tensor([1.0, 0.5, -0.5, 0.25, 1 / 3] + [0.0] * 11, device=cuda)).to(dt)
+        q, s = ops.quant_s8(x)
+        xf = np_(x.float())
+        want = (np.abs(xf).max(1) / np.float32(127)).astype(np.float32)
+        assert np.array_equal(np_(q), np.rint((xf / want[:, None]).astype(np.float32)).astype(np.int8))
 
 
 def test_no_rows_and_other_stream(cuda):

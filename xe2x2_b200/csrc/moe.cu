@@ -337,31 +337,95 @@ __device__ __forceinline__ T from_f(float v) {
     else return Conv<T>::from_f(v);
 }
 
-template <typename TY, typename TO>
-__global__ void __launch_bounds__(256) combine_kernel(const TY *__restrict__ y, int rows, const int *__restrict__ slots,
-                                                      const float *__restrict__ weights, const TO *add, TO *out, int k,
-                                                      int H) {
+template <typename T, int N>
+__device__ __forceinline__ void load_n(const T *p, float (&v)[N]) {
+    if constexpr (N == 1) {
+        v[0] = as_f<T>(*p);
+    } else {
+        constexpr int W = N * (int)sizeof(T) / 4;  // 32-bit words, a multiple of 2
+        uint32_t w[W];
+#pragma unroll
+        for (int i = 0; i < W; i += W % 4 ? 2 : 4) {
+            if constexpr (W % 4 == 0) {
+                const uint4 u = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint32_t *>(p) + i);
+                w[i] = u.x, w[i + 1] = u.y, w[i + 2] = u.z, w[i + 3] = u.w;
+            } else {
+                const uint2 u = *reinterpret_cast<const uint2 *>(reinterpret_cast<const uint32_t *>(p) + i);
+                w[i] = u.x, w[i + 1] = u.y;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if constexpr (sizeof(T) == 4) {
+                v[i] = __uint_as_float(w[i]);
+            } else {
+                const float2 f = Conv<T>::to_f2(w[i / 2]);
+                v[i] = i & 1 ? f.y : f.x;
+            }
+        }
+    }
+}
+
+// N channels a thread (16 bytes of y, or one where rows cannot be read that way), eight choices' rows
+// in flight.  Bound by memory: top_k + 1 rows a token.
+constexpr int kCombineThreads = 128;
+template <typename TY, typename TO, int N>
+__global__ void __launch_bounds__(kCombineThreads)
+combine_kernel(const TY *__restrict__ y, int rows, const int *__restrict__ slots, const float *__restrict__ weights,
+               const TO *add, TO *out, int k, int H) {
     grid_dep_launch();
     grid_dep_wait();
-    const int t = blockIdx.x;
-    for (int h = blockIdx.y * 256 + threadIdx.x; h < H; h += gridDim.y * 256) {
-        float acc = add ? as_f<TO>(add[(size_t)t * H + h]) : 0.f;
-        for (int j = 0; j < k; ++j) {
-            const int s = slots[(size_t)t * k + j];
-            const float v = s >= 0 && s < rows ? as_f<TY>(y[(size_t)s * H + h]) : 0.f;
-            acc = fmaf(weights[(size_t)t * k + j], v, acc);
+    const size_t t = blockIdx.x;
+    const int h = (blockIdx.y * kCombineThreads + threadIdx.x) * N;
+    if (h >= H) return;
+    float acc[N] = {};
+    if (add) load_n<TO, N>(add + t * H + h, acc);
+    for (int j0 = 0; j0 < k; j0 += 8) {
+        float v[8][N], w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const bool on = j0 + j < k;
+            const int s = on ? slots[t * k + j0 + j] : -1;
+            w[j] = on ? weights[t * k + j0 + j] : 0.f;
+            if (s >= 0 && s < rows) {
+                load_n<TY, N>(y + (size_t)s * H + h, v[j]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i) v[j][i] = 0.f;
+            }
         }
-        out[(size_t)t * H + h] = from_f<TO>(acc);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[i] = fmaf(w[j], v[j][i], acc[i]);
+    }
+    TO *dst = out + t * H + h;
+    if constexpr (N == 1) {
+        *dst = from_f<TO>(acc[0]);
+    } else {
+        __align__(16) TO r[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) r[i] = from_f<TO>(acc[i]);
+        if constexpr (N * sizeof(TO) % 16 == 0) {
+#pragma unroll
+            for (int i = 0; i < N * (int)sizeof(TO) / 16; ++i)
+                reinterpret_cast<uint4 *>(dst)[i] = reinterpret_cast<const uint4 *>(r)[i];
+        } else {
+            *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<const uint2 *>(r);
+        }
     }
 }
 
 template <typename TY, typename TO>
 static int launch_combine(const void *y, int rows, const int *slots, const float *weights, const void *add, void *out,
                           int T, int k, int H, cudaStream_t st) {
-    const int gy = (H + 255) / 256;
-    W4_CUDA_TRY(launch_decode(combine_kernel<TY, TO>, dim3(T, gy < 32 ? gy : 32), dim3(256), 0, st, 1,
-                              static_cast<const TY *>(y), rows, slots, weights, static_cast<const TO *>(add),
-                              static_cast<TO *>(out), k, H));
+    constexpr int N = 16 / (int)sizeof(TY);
+    const bool wide = H % N == 0 && aligned(y, 16) && aligned(out, 16) && aligned(add, 16);
+    const int per = kCombineThreads * (wide ? N : 1), gy = (H + per - 1) / per;
+    W4_REQUIRE(gy <= 65535, W4_ERR_UNSUPPORTED, "H=%d is too long", H);
+    W4_CUDA_TRY(launch_decode(wide ? combine_kernel<TY, TO, N> : combine_kernel<TY, TO, 1>, dim3(T, gy),
+                              dim3(kCombineThreads), 0, st, 1, static_cast<const TY *>(y), rows, slots, weights,
+                              static_cast<const TO *>(add), static_cast<TO *>(out), k, H));
     return W4_OK;
 }
 
