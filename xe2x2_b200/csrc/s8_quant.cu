@@ -12,40 +12,69 @@ namespace s8q {
 
 constexpr uint32_t kInfBits = 0x7F800000u;
 
-// Eight consecutive values of a row, 16-byte loads.
-template <typename T>
-__device__ __forceinline__ void load8(const T *p, float (&v)[8]) {
-    if constexpr (sizeof(T) == 4) {
-        const uint4 a = ld_nc_v4(p), b = ld_nc_v4(p + 4);
-        const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+// Eight consecutive values of a row: 16-byte loads, and their values.
+template <typename T> struct Raw8 {
+    static constexpr int W = 2 * (int)sizeof(T);  // 32-bit words
+    uint32_t w[W];
+    __device__ __forceinline__ void load(const T *p) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
-    } else {
-        const uint4 a = ld_nc_v4(p);
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = Conv<T>::to_f2(w[i]);
-            v[2 * i] = f.x;
-            v[2 * i + 1] = f.y;
+        for (int i = 0; i < W; i += 4) {
+            const uint4 u = ld_nc_v4(reinterpret_cast<const uint32_t *>(p) + i);
+            w[i] = u.x, w[i + 1] = u.y, w[i + 2] = u.z, w[i + 3] = u.w;
         }
     }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[i] = 0u;
+    }
+    __device__ __forceinline__ void values(float (&v)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (sizeof(T) == 4) {
+                v[i] = __uint_as_float(w[i]);
+            } else {
+                const float2 f = Conv<T>::to_f2(w[i / 2]);
+                v[i] = i & 1 ? f.y : f.x;
+            }
+        }
+    }
+};
+
+// g / (1 + exp(-g)) with the hardware's base-2 exponential (relative error 2^-22, and that of its rounded
+// argument, |g| 2^-24) and reciprocal (2^-23; 0 where the exponential is infinite or near it): about
+// 6e-7 for |g| up to 8, a thousandth of a code.  expf and a division made this kernel bound by its
+// instructions (37 a value, 60 us where this takes 45).
+__device__ __forceinline__ float silu(float g) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+    return g * r;
 }
 
-template <typename T, int FN>
-__device__ __forceinline__ void load_y(const T *xr, int K, int j, float (&y)[8]) {
-    load8(xr + j, y);
-    if constexpr (FN == W4_FN_SILU_MUL) {
-        float u[8];
-        load8(xr + K + j, u);
-        // __fdividef: within 2 ulp; 0 where the exponential overflows
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = __fdividef(y[i], 1.f + expf(-y[i])) * u[i];
-    } else if constexpr (FN == W4_FN_RELU2) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = y[i] < 0.f ? 0.f : y[i] * y[i];  // NaN stays NaN
+// Eight inputs of fn (with SwiGLU: of the gate and of the up half) and fn of them.
+template <typename T, int FN> struct In8 {
+    Raw8<T> a, b;
+    __device__ __forceinline__ void load(const T *xr, int K, int j) {
+        a.load(xr + j);
+        if constexpr (FN == W4_FN_SILU_MUL) b.load(xr + K + j);
     }
-}
+    __device__ __forceinline__ void zero() {
+        a.zero();
+        if constexpr (FN == W4_FN_SILU_MUL) b.zero();
+    }
+    __device__ __forceinline__ void values(float (&y)[8]) const {
+        a.values(y);
+        if constexpr (FN == W4_FN_SILU_MUL) {
+            float u[8];
+            b.values(u);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = silu(y[i]) * u[i];
+        } else if constexpr (FN == W4_FN_RELU2) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = y[i] < 0.f ? 0.f : y[i] * y[i];  // NaN stays NaN
+        }
+    }
+};
 
 // max(|a|, |b|, |c|), NaN if one is.
 __device__ __forceinline__ float absmax3(float a, float b, float c) {
@@ -107,46 +136,54 @@ __device__ __forceinline__ uint2 quant8(const float (&y)[8], const Scale &c) {
 }
 
 // A row on TPR threads, held in registers from the one read to the store: VPT vectors of eight values a
-// thread.  Bound by memory (5 bytes a value with SwiGLU); at 24,576 x 1856, bf16 -> 47 us, 4.9 TB/s,
-// where one CTA a row with a second read took 139.
+// thread.  CTAs loop over rows, and a row's loads are issued before the row ahead of it is reduced
+// (not with 1024 threads, whose registers are taken).  Bound by memory (5 bytes a value with SwiGLU)
+// and the instructions per value about equally; at 24,576 x 1856, bf16 -> 45 us, 5.0 TB/s, where
+// one CTA a row with a second read and a division per value took 139.
 template <typename T, int FN, int TPR, int VPT>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
 quant_s8_kernel(const T *__restrict__ x, int8_t *__restrict__ q, float *__restrict__ scale, int M, int K) {
     constexpr int RPC = TPR < 256 ? 256 / TPR : 1;  // rows of a CTA
-    __shared__ uint32_t sh[RPC][TPR / 32];
+    constexpr bool AHEAD = TPR < 1024;
+    __shared__ uint32_t sh[2][RPC][TPR / 32];
     grid_dep_launch();
     grid_dep_wait();
     const int rl = threadIdx.x / TPR, t = threadIdx.x % TPR;
-    const long row = (long)blockIdx.x * RPC + rl;
-    const bool in = row < M;
-    const T *xr = x + (size_t)row * K * (FN == W4_FN_SILU_MUL ? 2 : 1);
-    float y[VPT][8];
+    const size_t width = (size_t)K * (FN == W4_FN_SILU_MUL ? 2 : 1);
+    In8<T, FN> in[VPT];
+    auto fetch = [&](long row) {
 #pragma unroll
-    for (int v = 0; v < VPT; ++v) {
-        const int j = (v * TPR + t) * 8;
-        if (in && j < K) {
-            load_y<T, FN>(xr, K, j, y[v]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[v][i] = 0.f;
+        for (int v = 0; v < VPT; ++v) {
+            const int j = (v * TPR + t) * 8;
+            if (row < M && j < K) in[v].load(x + row * width, K, j);
+            else in[v].zero();
         }
-    }
-    float most = 0.f;
+    };
+    long row = (long)blockIdx.x * RPC + rl;
+    if (AHEAD) fetch(row);
+    // all rows of the CTA take the same number of turns
+    for (int turn = 0; row - rl < M; row += (long)gridDim.x * RPC, turn ^= 1) {
+        if (!AHEAD) fetch(row);
+        float y[VPT][8], most = 0.f;
 #pragma unroll
-    for (int v = 0; v < VPT; ++v) most = absmax8(y[v], most);
-    uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
-    if constexpr (TPR > 32) {
-        if ((t & 31) == 0) sh[rl][t / 32] = top;
-        __syncthreads();
-        top = __reduce_max_sync(0xffffffffu, (t & 31) < TPR / 32 ? sh[rl][t & 31] : 0u);
-    }
-    const Scale c = scale_of(top);
-    if (!in) return;
-    if (t == 0) scale[row] = c.s;
+        for (int v = 0; v < VPT; ++v) in[v].values(y[v]);
+        if (AHEAD) fetch(row + (long)gridDim.x * RPC);
 #pragma unroll
-    for (int v = 0; v < VPT; ++v) {
-        const int j = (v * TPR + t) * 8;
-        if (j < K) *reinterpret_cast<uint2 *>(q + (size_t)row * K + j) = quant8(y[v], c);
+        for (int v = 0; v < VPT; ++v) most = absmax8(y[v], most);
+        uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+        if constexpr (TPR > 32) {
+            if ((t & 31) == 0) sh[turn][rl][t / 32] = top;
+            __syncthreads();
+            top = __reduce_max_sync(0xffffffffu, (t & 31) < TPR / 32 ? sh[turn][rl][t & 31] : 0u);
+        }
+        if (row >= M) continue;
+        const Scale c = scale_of(top);
+        if (t == 0) scale[row] = c.s;
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+            const int j = (v * TPR + t) * 8;
+            if (j < K) *reinterpret_cast<uint2 *>(q + (size_t)row * K + j) = quant8(y[v], c);
+        }
     }
 }
 
@@ -162,7 +199,9 @@ quant_s8_long_kernel(const T *__restrict__ x, int8_t *__restrict__ q, float *__r
     float most = 0.f;
     for (int j = threadIdx.x * 8; j < K; j += 1024 * 8) {
         float y[8];
-        load_y<T, FN>(xr, K, j, y);
+        In8<T, FN> in;
+        in.load(xr, K, j);
+        in.values(y);
         most = absmax8(y, most);
     }
     uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
@@ -173,20 +212,23 @@ quant_s8_long_kernel(const T *__restrict__ x, int8_t *__restrict__ q, float *__r
     if (threadIdx.x == 0) scale[row] = c.s;
     for (int j = threadIdx.x * 8; j < K; j += 1024 * 8) {
         float y[8];
-        load_y<T, FN>(xr, K, j, y);
+        In8<T, FN> in;
+        in.load(xr, K, j);
+        in.values(y);
         *reinterpret_cast<uint2 *>(q + row * K + j) = quant8(y, c);
     }
 }
 
 template <typename T, int FN, int TPR, int VPT>
 static int launch(const T *x, int8_t *q, float *scale, int M, int K, cudaStream_t st) {
-    constexpr int RPC = TPR < 256 ? 256 / TPR : 1;
-    W4_CUDA_TRY(launch_decode(quant_s8_kernel<T, FN, TPR, VPT>, dim3((M + RPC - 1) / RPC), dim3(TPR < 256 ? 256 : TPR), 0,
-                              st, 1, x, q, scale, M, K));
+    constexpr int CTA = TPR < 256 ? 256 : TPR, RPC = CTA / TPR;
+    const int ctas = (M + RPC - 1) / RPC, room = num_sms() * (1536 / CTA);  // 1024 threads an SM: 49 us, 1536: 45
+    W4_CUDA_TRY(launch_decode(quant_s8_kernel<T, FN, TPR, VPT>, dim3(ctas < room || TPR == 1024 ? ctas : room), dim3(CTA),
+                              0, st, 1, x, q, scale, M, K));
     return W4_OK;
 }
 
-// Threads a row: a power of two with at most two vectors a thread up to 1024 threads, then four.
+// Threads a row: a power of two with at most two vectors a thread up to 1024 threads, then three or four.
 template <typename T, int FN>
 static int launch_fn(const void *xv, int8_t *q, float *scale, int M, int K, cudaStream_t st) {
     const T *x = static_cast<const T *>(xv);
@@ -197,6 +239,7 @@ static int launch_fn(const void *xv, int8_t *q, float *scale, int M, int K, cuda
     if (nvec <= 512) return launch<T, FN, 256, 2>(x, q, scale, M, K, st);
     if (nvec <= 1024) return launch<T, FN, 512, 2>(x, q, scale, M, K, st);
     if (nvec <= 2048) return launch<T, FN, 1024, 2>(x, q, scale, M, K, st);
+    if (nvec <= 3 * 1024) return launch<T, FN, 1024, 3>(x, q, scale, M, K, st);
     if (nvec <= 4096) return launch<T, FN, 1024, 4>(x, q, scale, M, K, st);
     W4_CUDA_TRY(launch_decode(quant_s8_long_kernel<T, FN>, dim3(M), dim3(1024), 0, st, 1, x, q, scale, K));
     return W4_OK;
