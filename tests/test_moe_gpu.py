@@ -67,11 +67,15 @@ def _check(logits, k, bias=None, score="softmax", renormalize=True, scaling=1.0,
     ids, w = _route64(logits, b, k, score, renormalize, scaling, n_group, topk_group, group_score)
     r = ops.moe_route(logits, k, bias, score, renormalize, scaling, n_group, topk_group, group_score)
     assert np.array_equal(np_(r.ids), ids)
-    # scores of the chosen and their sum are taken in 64 bits; without renormalising the softmax's
-    # sum may be in 32: E terms of expf (1 ulp = 2^-23, and its argument's rounding, at most
-    # |x| 2^-24 with |x| < 32 where a term counts) and their additions; then the store rounds
+    # In 32 bits: expf within 1 ulp (2^-23) of its argument, which rounds by at most |x| 2^-24 (x the
+    # logit under the softmax's largest; logits here are below 32 in size where a weight counts), 1 + e and
+    # the quotient (2^-24 each); the same again in the sum, plus its additions (5), and the last quotient,
+    # the scaling and the store.  Without renormalising the softmax's sum has E terms of its own, with the
+    # base-2 exponential (2^-22).
     E = logits.shape[1]
-    rel = 2.0 ** -24 + 1e-12 + (0 if renormalize or score != "softmax" else 2.0 ** -23 + 32 * 2.0 ** -24 + E * 2.0 ** -24)
+    rel = 2 * (2 * 32 * 2.0 ** -24 if score == "softmax" else 0) + 16 * 2.0 ** -24
+    if not renormalize and score == "softmax":
+        rel += 2.0 ** -22 + E * 2.0 ** -24
     got = np_(r.weights).astype(np.float64)
     assert np.array_equal(np.isnan(got), np.isnan(w))
     fine = ~np.isnan(w)

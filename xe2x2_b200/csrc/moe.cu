@@ -17,8 +17,11 @@ namespace moe {
 // are unsigned integers that order as the values do, 0 for an expert that cannot be chosen, and
 // the warp's maximum is one redux (32-bit keys) or two (64-bit).  Without a bias the order of the
 // scores is the order of the logits and the key is the logit, exact in 32 bits.  With one the key
-// is score + bias in 64 bits: the k-th and the next score of a few thousand tokens come closer
-// than 32 bits tell apart, and the choice would then depend on how exp was rounded.
+// is score + bias, and the k-th and the next score of a few thousand tokens come closer than 32 bits
+// tell apart: the choice would depend on how exp was rounded.  So a token is first chosen for in 32
+// bits, with one rank more than asked for, and where two neighbours (or the last group kept and the
+// next) are closer than the 32-bit errors, it is chosen for again in 64 (under 1 % of the tokens; all
+// in 64 bits took 61 us for 8192 x 256, top 8 of 4 in 8 groups, where this takes FIGURE).
 //
 // The order by expert is a counting sort without atomics whose order matters: a token takes an
 // expert at most once, so a bit mask over a chunk's tokens for each expert gives counts (popc) and
@@ -29,12 +32,14 @@ struct RouteArgs {
     const void *logits;
     const float *bias;
     int dtype, T, E, k, softmax, groups, topk_group, top2, renorm;
+    int whole;  // lanes of a group, where that is a whole power of two, else 0
     float scaling;
     int *ids;
     float *weights;
     int *offsets, *rows, *slots;  // null: no plan
-    int *counts;                  // [chunks][E], null with one chunk
-    int chunk;                    // tokens per CTA, a multiple of 32
+    uint16_t *counts;             // [E][chunks, padded to 8 with zeros], null with one chunk
+    int chunk, words;             // tokens per CTA, and words of their bit masks
+    bool vec, vec_bias;           // a lane's logits, its biases, are aligned to their size or 16
 };
 
 __device__ __forceinline__ float load_logit(const void *p, int dt, size_t i) {
@@ -43,14 +48,18 @@ __device__ __forceinline__ float load_logit(const void *p, int dt, size_t i) {
     return __half2float(static_cast<const __half *>(p)[i]);
 }
 
+__device__ __forceinline__ float logit_of(const RouteArgs &a, int t, int e) {
+    return load_logit(a.logits, a.dtype, (size_t)t * a.E + e);
+}
+
 // Unsigned integers in the order of the values; above 0 for every value but -NaN.
 __device__ __forceinline__ uint32_t ordered(float v) {
-    const uint32_t b = __float_as_uint(v);
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
+    const int b = __float_as_int(v);
+    return (uint32_t)(b ^ ((b >> 31) | (int)0x80000000));
 }
 __device__ __forceinline__ uint64_t ordered(double v) {
-    const uint64_t b = (uint64_t)__double_as_longlong(v);
-    return b >> 63 ? ~b : b | 0x8000000000000000ull;
+    const long long b = __double_as_longlong(v);
+    return (uint64_t)(b ^ ((b >> 63) | (long long)0x8000000000000000ull));
 }
 __device__ __forceinline__ uint32_t warp_max(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
 __device__ __forceinline__ uint64_t warp_max(uint64_t v) {
@@ -64,135 +73,412 @@ __device__ __forceinline__ double warp_sum(double v) {
     return v;
 }
 
-__device__ __forceinline__ double score_of(float l, bool softmax, float top) {
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+__device__ __forceinline__ float from_ordered(uint32_t k) {
+    return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
+}
+
+// exp(l - top) or 1 / (1 + exp(-l)): in 64 bits, and in 32 with the hardware's base-2 exponential and
+// reciprocal.
+__device__ __forceinline__ double score_of(float l, bool softmax, float top, double) {
     return softmax ? exp((double)l - (double)top) : 1.0 / (1.0 + exp(-(double)l));
 }
-
-// Bit mask of the groups whose experts may be chosen: lane g sums up group g.
-__device__ __forceinline__ uint32_t kept_groups(const double *base, const RouteArgs &a, int lane) {
-    const int size = a.E / a.groups;
-    double first = -HUGE_VAL, second = -HUGE_VAL;
-    if (lane < a.groups)
-        for (int i = 0; i < size; ++i) {
-            const double v = base[lane * size + i];
-            if (v > first) {
-                second = first;
-                first = v;
-            } else if (v > second) {
-                second = v;
-            }
-        }
-    const double total = a.top2 && second > -HUGE_VAL ? first + second : first;
-    int rank = 0;
-    for (int g = 0; g < a.groups; ++g) {
-        const double o = __shfl_sync(0xffffffffu, total, g);
-        rank += o > total || (o == total && g < lane);
-    }
-    return __ballot_sync(0xffffffffu, lane < a.groups && rank < a.topk_group);
+__device__ __forceinline__ float score_of(float l, bool softmax, float top, float) {
+    constexpr float kLog2e = 1.4426950408889634f;
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((softmax ? l - top : -l) * kLog2e));
+    if (softmax) return e;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+    return r;
+}
+// Two values further apart than this are in order although their scores were taken in 32 bits.  A sigmoid
+// of 32 bits is within 2e-7 of the exact one (2^-22 of the exponential times at most a quarter, 2^-23 of
+// the reciprocal); a softmax's terms are within 3e-6 of their size (argument and exponential, and a sum
+// of up to 512 terms).  `score` is the larger score (or sum of scores) of the two; their values round
+// once or twice more.
+__device__ __forceinline__ float close_to(bool softmax, float score, float value) {
+    return (softmax ? 6e-6f * score : 1e-6f) + 5e-7f * fabsf(value);
 }
 
+// What a warp knows of one token: its logits (-inf where an expert is off), the largest one (finite), and
+// the logits' keys (0 where an expert is off).
+template <int EPL> struct Token {
+    float l[EPL], top;
+    uint32_t key[EPL];
+    bool live, nan;
+    int t;
+};
+struct Choice {
+    int e;     // lane j: the j-th expert, -1 if there is none
+    double z;  // the softmax's sum, where it was needed
+};
+
+__device__ __forceinline__ int padded(int e) { return e + (e >> 5); }  // apart in the banks from group to group
+
+// The two largest values of `n` neighbouring lanes (a power of two), from each lane's two.
+template <typename V>
+__device__ __forceinline__ void merge_top2(V &first, V &second, int n) {
+    for (int o = 1; o < n; o <<= 1) {
+        const V f = __shfl_xor_sync(0xffffffffu, first, o), s = __shfl_xor_sync(0xffffffffu, second, o);
+        const V least = first < f ? first : f;
+        second = f > first ? s : second;
+        first = f > first ? f : first;
+        second = second > least ? second : least;
+    }
+}
+template <typename V>
+__device__ __forceinline__ void add_top2(V &first, V &second, V v) {
+    const V least = v < first ? v : first;
+    first = v > first ? v : first;
+    second = least > second ? least : second;
+}
+
+// Whether this lane's group (lpg neighbouring lanes hold one, with its two best values) is among those
+// whose experts may be chosen.  *close: whether 32-bit errors could have swapped the last group in for
+// the first one out.
+template <typename V>
+__device__ __forceinline__ bool group_kept(const RouteArgs &a, V first, V second, int lpg, int lane, bool *close) {
+    const int g = lane / lpg;
+    const V total = a.top2 && second > (V)-INFINITY ? first + second : first;
+    int rank = 0;
+    for (int o = 0; o < a.groups; ++o) {
+        const V v = __shfl_sync(0xffffffffu, total, o * lpg);
+        rank += v > total || (v == total && o < g);
+    }
+    if (close && a.topk_group < a.groups) {
+        const bool lead = lane % lpg == 0 && g < a.groups;
+        const int in = __ffs(__ballot_sync(0xffffffffu, lead && rank == a.topk_group - 1)) - 1;
+        const int out = __ffs(__ballot_sync(0xffffffffu, lead && rank == a.topk_group)) - 1;
+        const float x = (float)__shfl_sync(0xffffffffu, total, in), y = (float)__shfl_sync(0xffffffffu, total, out);
+        *close = y > -INFINITY && x - y <= 2 * close_to(a.softmax, 1.f, x);
+    }
+    return g < a.groups && rank < a.topk_group;
+}
+
+// The largest key of the warp: its expert in every lane, and the key taken off.  0: none left.
 template <int EPL, typename KeyT>
-__device__ __forceinline__ void route_token(const RouteArgs &a, int t, double *base, uint32_t *mask, int words,
-                                            int t_local) {
+__device__ __forceinline__ KeyT take_best(KeyT (&key)[EPL], int lane, int *e) {
+    KeyT best = key[0];
+#pragma unroll
+    for (int i = 1; i < EPL; ++i) best = max(best, key[i]);
+    const KeyT m = warp_max(best);
+    if (m == 0) return 0;
+    const int win = __ffs(__ballot_sync(0xffffffffu, best == m)) - 1;
+    int at = 0;
+#pragma unroll
+    for (int i = EPL - 1; i > 0; --i)
+        if (key[i] == m) at = i;
+    if (key[0] == m) at = 0;
+    *e = __shfl_sync(0xffffffffu, lane * EPL + at, win);
+#pragma unroll
+    for (int i = 0; i < EPL; ++i)
+        if (lane * EPL + i == *e) key[i] = 0;
+    return m;
+}
+
+// EPL floats in a row, in 16-byte loads (aligned to their size or 16).
+template <int EPL>
+__device__ __forceinline__ void load_f32(const float *p, float (&v)[EPL]) {
+    if constexpr (EPL >= 4) {
+#pragma unroll
+        for (int i = 0; i < EPL; i += 4) {
+            const float4 u = *reinterpret_cast<const float4 *>(p + i);
+            v[i] = u.x, v[i + 1] = u.y, v[i + 2] = u.z, v[i + 3] = u.w;
+        }
+    } else if constexpr (EPL == 2) {
+        const float2 u = *reinterpret_cast<const float2 *>(p);
+        v[0] = u.x, v[1] = u.y;
+    } else {
+        v[0] = *p;
+    }
+}
+
+// A warp's scratch for select32: the lanes' maxima, candidates and the order (key, expert).
+struct Pick {
+    uint32_t best[32];
+    uint2 cand[32], out[32];
+};
+
+// The kk <= 32 largest keys in order, the j-th to lane j (*m = 0 where there is none), in a fixed number
+// of steps: the kk-th largest of the lanes' maxima bounds the kk-th largest key from below, and the
+// few keys from there on are ranked against each other.  False if those are more than 32.
+template <int EPL>
+__device__ __forceinline__ bool select32(const uint32_t (&key)[EPL], int kk, int lane, Pick *p, int *e, uint32_t *m) {
+    uint32_t best = key[0];
+#pragma unroll
+    for (int i = 1; i < EPL; ++i) best = max(best, key[i]);
+    p->best[lane] = best;
+    __syncwarp();
+    int above = 0;
+#pragma unroll
+    for (int o = 0; o < 32; o += 4) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(p->best + o);
+        above += (v.x > best) + (v.y > best) + (v.z > best) + (v.w > best);
+    }
+    const uint32_t least = max(__reduce_min_sync(0xffffffffu, above < kk ? best : 0xffffffffu), 1u);
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+        const bool in = key[i] >= least;
+        const uint32_t b = __ballot_sync(0xffffffffu, in);
+        const int pos = n + __popc(b & ((1u << lane) - 1));
+        if (in && pos < 32) p->cand[pos] = make_uint2(key[i], lane * EPL + i);
+        n += __popc(b);
+    }
+    __syncwarp();
+    if (n > 32) return false;
+    const uint2 mine = lane < n ? p->cand[lane] : make_uint2(0u, 0u);
+    int rank = 0;
+#pragma unroll 4
+    for (int c = 0; c < n; ++c) {
+        const uint2 o = p->cand[c];
+        rank += o.x > mine.x || (o.x == mine.x && o.y < mine.y);
+    }
+    if (lane < n) p->out[rank] = mine;
+    __syncwarp();
+    const bool on = lane < n && lane < kk;
+    const uint2 r = on ? p->out[lane] : make_uint2(0u, 0u);
+    *m = r.x;
+    *e = on ? (int)r.y : -1;
+    return true;
+}
+
+// Choose for a token with values of type V (float or double).  False: too close to call in 32 bits.
+template <int EPL, typename V, typename KeyT>
+__device__ __forceinline__ bool choose(const RouteArgs &a, const Token<EPL> &k, V *base, int lpg, Pick *pick, int lane,
+                                       Choice *c) {
+    constexpr bool NARROW = sizeof(V) == 4;
+    const bool scored = a.bias || (a.groups > 1 && a.top2);  // values that are compared are not all logits
+    const bool doubt = NARROW && scored;
+    KeyT key[EPL];
+    V val[EPL];  // what groups are scored by
+    if (!scored) {
+        if (a.softmax && !a.renorm) {  // the weights need the sum
+            V z = 0;
+#pragma unroll
+            for (int i = 0; i < EPL; ++i)
+                if (k.key[i]) z += score_of(fminf(k.l[i], FLT_MAX), true, k.top, V());
+            c->z = (double)warp_sum(z);
+        }
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) key[i] = k.key[i];
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) val[i] = (V)k.l[i];
+    } else {
+        V (&s)[EPL] = val, z = 0;
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) {
+            s[i] = 0;
+            if (k.key[i]) s[i] = score_of(fminf(k.l[i], FLT_MAX), a.softmax, k.top, V());
+            z += s[i];
+        }
+        if (a.softmax) {
+            z = warp_sum(z);
+            c->z = (double)z;
+            if (k.live) {
+                const V iz = (V)1 / z;
+#pragma unroll
+                for (int i = 0; i < EPL; ++i) s[i] = NARROW ? s[i] * iz : s[i] / z;
+            }
+        }
+        if (a.bias) {
+            float b[EPL];
+            if (a.vec_bias && lane * EPL < a.E) {
+                load_f32<EPL>(a.bias + lane * EPL, b);
+            } else {
+#pragma unroll
+                for (int i = 0; i < EPL; ++i) b[i] = lane * EPL + i < a.E ? a.bias[lane * EPL + i] : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) {
+                s[i] += (V)b[i];
+                key[i] = k.key[i] && s[i] > (V)-INFINITY ? ordered(s[i] + (V)0) : 0;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) key[i] = NARROW ? k.key[i] : k.key[i] ? ordered((V)k.l[i]) : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) val[i] = key[i] ? s[i] : (V)-INFINITY;
+    }
+    if (a.groups > 1) {
+        const V low = (V)-INFINITY;
+        V first = low, second = low;
+        bool close = false;
+        if (a.whole) {  // a group is a power of two of whole lanes
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) add_top2(first, second, val[i]);
+            merge_top2(first, second, a.whole);
+            const bool kept = group_kept<V>(a, first, second, a.whole, lane, doubt ? &close : nullptr);
+            if (close) return false;
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) key[i] = kept ? key[i] : 0;
+        } else {
+#pragma unroll
+            for (int i = 0; i < EPL; ++i)
+                if (lane * EPL + i < a.E) base[padded(lane * EPL + i)] = val[i];
+            __syncwarp();
+            const int size = a.E / a.groups, mine = lane / lpg;
+            if (mine < a.groups)
+                for (int i = lane % lpg; i < size; i += lpg) add_top2(first, second, base[padded(mine * size + i)]);
+            __syncwarp();  // base is rewritten later
+            merge_top2(first, second, lpg);
+            const bool in = group_kept<V>(a, first, second, lpg, lane, doubt ? &close : nullptr);
+            const uint32_t kept = __ballot_sync(0xffffffffu, in);
+            if (close) return false;
+            int g = lane * EPL / size, r = lane * EPL % size;
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) {
+                if (lane * EPL + i < a.E && !(kept >> (g * lpg) & 1)) key[i] = 0;
+                if (++r == size) {
+                    r = 0;
+                    ++g;
+                }
+            }
+        }
+    }
+    c->e = -1;
+    KeyT mine = 0;  // lane j: the j-th key; in doubt also the one behind the last
+    uint32_t last = 0;
+    int last_e = -1;
+    bool done = false;
+    if constexpr (NARROW) {
+        const int kk = a.k + (doubt && a.bias ? 1 : 0);
+        if (kk <= 32 && select32<EPL>(key, kk, lane, pick, &c->e, &mine)) {
+            done = true;
+            last = __shfl_sync(0xffffffffu, mine, a.k & 31);
+            last_e = __shfl_sync(0xffffffffu, c->e, a.k & 31);
+            if (kk == a.k) last = 0;
+        }
+    }
+    if (!done) {
+        for (int j = 0; j <= a.k; ++j) {
+            int e = -1;
+            const KeyT m = take_best<EPL, KeyT>(key, lane, &e);
+            if (m == 0) break;  // nothing left to choose
+            if (j == a.k) {
+                last = (uint32_t)m;
+                last_e = e;
+            } else if (lane == j) {
+                c->e = e;
+                mine = m;
+            }
+        }
+    }
+    if (lane >= a.k) c->e = -1;
+    if constexpr (NARROW) {
+        if (a.bias) {  // are all neighbours in the order, the one behind it included, clearly apart?
+            const int be = __shfl_down_sync(0xffffffffu, c->e, 1);
+            const uint32_t bm = __shfl_down_sync(0xffffffffu, mine, 1);
+            const int e2 = lane == a.k - 1 ? last_e : be;
+            const uint32_t m2 = lane == a.k - 1 ? last : bm;
+            bool near = false;
+            if (lane < a.k && c->e >= 0 && m2 != 0 && e2 >= 0) {
+                const float x = from_ordered(mine), y = from_ordered(m2), bx = a.bias[c->e], by = a.bias[e2];
+                // equal logits and biases are a tie in any precision
+                if (x - y <= close_to(a.softmax, fmaxf(x - bx, y - by), x))
+                    near = bx != by || logit_of(a, k.t, c->e) != logit_of(a, k.t, e2);
+            }
+            if (__any_sync(0xffffffffu, near)) return false;
+        }
+    }
+    return true;
+}
+
+// Logits of a lane, EPL in a row: in one or a few wide loads where rows allow it.
+template <int EPL>
+__device__ __forceinline__ void load_logits(const RouteArgs &a, int t, int lane, float (&l)[EPL]) {
+    const size_t o = (size_t)t * a.E + lane * EPL;
+    if (a.vec && lane * EPL < a.E) {
+        if (a.dtype == W4_F32) {
+            load_f32<EPL>(static_cast<const float *>(a.logits) + o, l);
+            return;
+        }
+        if constexpr (EPL >= 2) {
+            const uint16_t *p = static_cast<const uint16_t *>(a.logits) + o;
+            uint32_t w[EPL / 2];
+            if constexpr (EPL >= 8) {
+#pragma unroll
+                for (int i = 0; i < EPL / 8; ++i) {
+                    const uint4 u = reinterpret_cast<const uint4 *>(p)[i];
+                    w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
+                }
+            } else if constexpr (EPL == 4) {
+                const uint2 u = *reinterpret_cast<const uint2 *>(p);
+                w[0] = u.x, w[1] = u.y;
+            } else {
+                w[0] = *reinterpret_cast<const uint32_t *>(p);
+            }
+#pragma unroll
+            for (int i = 0; i < EPL / 2; ++i) {
+                const float2 f = a.dtype == W4_BF16 ? Conv<__nv_bfloat16>::to_f2(w[i]) : Conv<__half>::to_f2(w[i]);
+                l[2 * i] = f.x;
+                l[2 * i + 1] = f.y;
+            }
+            return;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) l[i] = lane * EPL + i < a.E ? load_logit(a.logits, a.dtype, o + i) : -INFINITY;
+}
+
+template <int EPL>
+__device__ __forceinline__ void route_token(const RouteArgs &a, int t, const float (&logits)[EPL], double *base, int lpg,
+                                            Pick *pick, uint32_t *mask, int words, int t_local) {
     const int lane = threadIdx.x & 31;
-    constexpr bool kWide = sizeof(KeyT) == 8;
-    float l[EPL];
+    Token<EPL> k;
+    k.t = t;
     bool nan = false;
     uint32_t top_key = 0;
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
-        const int e = lane * EPL + i;
-        float v = e < a.E ? load_logit(a.logits, a.dtype, (size_t)t * a.E + e) : -INFINITY;
-        if (v != v) {
-            nan = true;
-            v = -INFINITY;
-        }
-        l[i] = v + 0.f;  // -0 orders as 0
-        if (v > -INFINITY) top_key = max(top_key, ordered(fminf(l[i], FLT_MAX)));
+        nan |= logits[i] != logits[i];
+        const bool on = logits[i] > -INFINITY;  // not for NaN
+        k.l[i] = on ? logits[i] : -INFINITY;
+        k.key[i] = on ? ordered(logits[i] + 0.f) : 0u;  // -0 orders as 0
+        top_key = max(top_key, k.key[i]);
     }
-    nan = __any_sync(0xffffffffu, nan);
+    k.nan = __any_sync(0xffffffffu, nan);
     top_key = warp_max(top_key);
-    const bool live = top_key != 0;
-    const float top = live ? __uint_as_float(top_key & 0x80000000u ? top_key & 0x7FFFFFFFu : ~top_key) : 0.f;
+    k.live = top_key != 0;
+    k.top = k.live ? fminf(from_ordered(top_key), FLT_MAX) : 0.f;
 
-    KeyT key[EPL];
-    double z = 0.0;  // sum of the softmax
-    if constexpr (kWide) {
-        double s[EPL];
-#pragma unroll
-        for (int i = 0; i < EPL; ++i) {
-            s[i] = l[i] > -INFINITY ? score_of(fminf(l[i], FLT_MAX), a.softmax, top) : 0.0;
-            z += s[i];
+    Choice c;
+    if (!choose<EPL, float, uint32_t>(a, k, reinterpret_cast<float *>(base), lpg, pick, lane, &c))
+        choose<EPL, double, uint64_t>(a, k, base, lpg, pick, lane, &c);
+
+    // Weights in 32 bits (the functions of the library, 1 ulp) unless a score is so small that it, or the
+    // sum, would be lost.
+    const float l = c.e >= 0 ? fminf(logit_of(a, t, c.e), FLT_MAX) : 0.f;
+    const float f = a.softmax ? expf(l - k.top) : __fdiv_rn(1.f, 1.f + expf(-l));
+    float w = c.e >= 0 ? f : 0.f;
+    if (__any_sync(0xffffffffu, c.e >= 0 && !(f > 1e-30f))) {
+        double d = c.e >= 0 ? score_of(l, a.softmax, k.top, 0.0) : 0.0;
+        if (a.renorm) {
+            const double sum = warp_sum(d);
+            d = sum > 0.0 ? d / sum : 0.0;
+        } else if (a.softmax && k.live) {
+            d /= c.z;
         }
-        z = warp_sum(z);
-#pragma unroll
-        for (int i = 0; i < EPL; ++i) {
-            const int e = lane * EPL + i;
-            const double p = a.softmax && live ? s[i] / z : s[i];
-            double v = a.bias ? (e < a.E ? p + (double)a.bias[e] : 0.0) : (double)l[i];
-            const bool off = !(l[i] > -INFINITY) || !(v > -HUGE_VAL);
-            key[i] = off ? 0 : ordered(v);
-            if (a.groups > 1 && e < a.E) base[e] = off ? -HUGE_VAL : a.top2 && !a.bias ? p : v;
-        }
+        w = (float)(d * (double)a.scaling);
     } else {
-        float zf = 0.f;
-#pragma unroll
-        for (int i = 0; i < EPL; ++i) {
-            const int e = lane * EPL + i;
-            if (a.softmax && !a.renorm && l[i] > -INFINITY) zf += expf(fminf(l[i], FLT_MAX) - top);
-            key[i] = l[i] > -INFINITY ? ordered(l[i]) : 0;
-            if (a.groups > 1 && e < a.E) base[e] = (double)l[i];
+        if (a.renorm) {
+            const float sum = warp_sum(w);
+            w = sum > 0.f ? __fdiv_rn(w, sum) : 0.f;
+        } else if (a.softmax && k.live) {
+            w = __fdiv_rn(w, (float)c.z);
         }
-        z = warp_sum((double)zf);
+        w *= a.scaling;
     }
-    if (a.groups > 1) {
-        __syncwarp();
-        const uint32_t kept = kept_groups(base, a, lane);
-        const int size = a.E / a.groups;
-#pragma unroll
-        for (int i = 0; i < EPL; ++i) {
-            const int e = lane * EPL + i;
-            if (e < a.E && !(kept >> (e / size) & 1)) key[i] = 0;
-        }
-        __syncwarp();  // base is rewritten for the next token
-    }
-
-    int my_e = -1;
-    float my_l = 0.f;
-    for (int j = 0; j < a.k; ++j) {
-        KeyT best = 0;
-        int at = 0;
-        float bl = 0.f;
-#pragma unroll
-        for (int i = 0; i < EPL; ++i)
-            if (key[i] > best) {
-                best = key[i];
-                at = i;
-                bl = l[i];
-            }
-        const KeyT m = warp_max(best);
-        if (m == 0) break;  // nothing left to choose
-        const int win = __ffs(__ballot_sync(0xffffffffu, best == m)) - 1;
-        const int e = __shfl_sync(0xffffffffu, lane * EPL + at, win);
-        const float wl = __shfl_sync(0xffffffffu, bl, win);
-        if (lane == j) {
-            my_e = e;
-            my_l = wl;
-        }
-#pragma unroll
-        for (int i = 0; i < EPL; ++i)
-            if (lane * EPL + i == e) key[i] = 0;
-    }
-
-    double w = my_e >= 0 ? score_of(fminf(my_l, FLT_MAX), a.softmax, top) : 0.0;
-    const double sum = warp_sum(w);
-    if (a.renorm) w = sum > 0.0 ? w / sum : 0.0;
-    else if (a.softmax && live) w /= z;
     if (lane < a.k) {
         const size_t o = (size_t)t * a.k + lane;
-        a.ids[o] = my_e;
-        a.weights[o] = nan ? __int_as_float(0x7fc00000) : (float)(w * (double)a.scaling);
-        if (a.offsets && my_e >= 0) atomicOr(&mask[my_e * words + (t_local >> 5)], 1u << (t_local & 31));
+        a.ids[o] = c.e;
+        a.weights[o] = k.nan ? __int_as_float(0x7fc00000) : w;
+        if (a.offsets && c.e >= 0) atomicOr(&mask[c.e * words + (t_local >> 5)], 1u << (t_local & 31));
     }
 }
 
@@ -248,28 +534,45 @@ __device__ __forceinline__ void place(const RouteArgs &a, const uint32_t *mask, 
         a.rows[i] = -1;
 }
 
-template <int EPL, typename KeyT>
-__global__ void __launch_bounds__(kThreads) route_kernel(const RouteArgs a) {
+template <int EPL>
+__global__ void __launch_bounds__(kThreads, EPL == 16 ? 1 : 2) route_kernel(const RouteArgs a) {
     extern __shared__ __align__(16) uint8_t sm[];
     __shared__ int base_sh[kMaxMoeExperts], scan_sh[kWarps];
-    const int words = a.chunk / 32;
+    __shared__ __align__(16) Pick pick_sh[kWarps];
+    const int words = a.words;
     uint32_t *mask = reinterpret_cast<uint32_t *>(sm);
     double *base = reinterpret_cast<double *>(sm + (((size_t)(a.offsets ? a.E * words : 0) * 4 + 15) & ~size_t(15))) +
-                   (size_t)(threadIdx.x >> 5) * a.E;
+                   (size_t)(threadIdx.x >> 5) * padded(a.E);
+    int lpg = 32;  // lanes that sum up a group: as many as every group can have
+    while (lpg * a.groups > 32) lpg >>= 1;
     grid_dep_launch();
     if (a.offsets)
         for (int i = threadIdx.x; i < a.E * words; i += kThreads) mask[i] = 0;
     __syncthreads();
     grid_dep_wait();
     const int t0 = blockIdx.x * a.chunk, n = min(a.chunk, a.T - t0);
-    for (int i = threadIdx.x >> 5; i < n; i += kWarps) route_token<EPL, KeyT>(a, t0 + i, base, mask, words, i);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float l[EPL], ahead[EPL];  // a token's logits are on their way while the one before it is chosen for
+    if (warp < n) load_logits<EPL>(a, t0 + warp, lane, ahead);
+    for (int i = warp; i < n; i += kWarps) {
+#pragma unroll
+        for (int u = 0; u < EPL; ++u) l[u] = ahead[u];
+        if (i + kWarps < n) load_logits<EPL>(a, t0 + i + kWarps, lane, ahead);
+        route_token<EPL>(a, t0 + i, l, base, lpg, &pick_sh[warp], mask, words, i);
+    }
     if (!a.offsets) return;
     __syncthreads();
     int count = 0;
     if ((int)threadIdx.x < a.E)
         for (int w = 0; w < words; ++w) count += __popc(mask[threadIdx.x * words + w]);
     if (a.counts) {
-        if ((int)threadIdx.x < a.E) a.counts[(size_t)blockIdx.x * a.E + threadIdx.x] = count;
+        const int pitch = (gridDim.x + 7) / 8 * 8;
+        if ((int)threadIdx.x < a.E) {
+            uint16_t *col = a.counts + (size_t)threadIdx.x * pitch;
+            col[blockIdx.x] = (uint16_t)count;  // at most 1024
+            if (blockIdx.x == gridDim.x - 1)
+                for (int c = gridDim.x; c < pitch; ++c) col[c] = 0;
+        }
     } else {
         place(a, mask, words, base_sh, scan_sh, t0, n, count, 0);
     }
@@ -278,7 +581,7 @@ __global__ void __launch_bounds__(kThreads) route_kernel(const RouteArgs a) {
 __global__ void __launch_bounds__(kThreads) place_kernel(const RouteArgs a) {
     extern __shared__ __align__(16) uint8_t sm[];
     __shared__ int base_sh[kMaxMoeExperts], scan_sh[kWarps];
-    const int words = a.chunk / 32;
+    const int words = a.words;
     uint32_t *mask = reinterpret_cast<uint32_t *>(sm);
     grid_dep_launch();
     for (int i = threadIdx.x; i < a.E * words; i += kThreads) mask[i] = 0;
@@ -289,35 +592,59 @@ __global__ void __launch_bounds__(kThreads) place_kernel(const RouteArgs a) {
         const int e = a.ids[(size_t)t0 * a.k + i], tl = i / a.k;
         if (e >= 0) atomicOr(&mask[e * words + (tl >> 5)], 1u << (tl & 31));
     }
-    int total = 0, before = 0;
-    if ((int)threadIdx.x < a.E)
+    // every chunk's counts, eight in 16 bytes: P threads an expert, then one
+    __shared__ int part_sh[2][kThreads];
+    int width = 32;
+    while (width < a.E) width <<= 1;  // at most kThreads
+    const int P = kThreads / width, e = threadIdx.x % width, c8 = (gridDim.x + 7) / 8;
+    unsigned total = 0, before = 0;
+    if (e < a.E) {
+        const uint4 *col = reinterpret_cast<const uint4 *>(a.counts) + (size_t)e * c8;
 #pragma unroll 8
-        for (int c = 0; c < (int)gridDim.x; ++c) {
-            const int v = a.counts[(size_t)c * a.E + threadIdx.x];
-            total += v;
-            if (c < (int)blockIdx.x) before += v;
+        for (int i = threadIdx.x / width; i < c8; i += P) {
+            const uint4 v = col[i];
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int c = 8 * i + 2 * u;  // chunks c and c + 1
+                total = __dp2a_lo(w[u], 0x0101u, total);
+                before = __dp2a_lo(w[u], (c < (int)blockIdx.x ? 1u : 0u) | (c + 1 < (int)blockIdx.x ? 0x100u : 0u),
+                                   before);
+            }
         }
+    }
+    part_sh[0][threadIdx.x] = total;
+    part_sh[1][threadIdx.x] = before;
     __syncthreads();
+    total = before = 0;
+    if ((int)threadIdx.x < a.E)
+        for (int i = 0; i < P; ++i) {
+            total += part_sh[0][i * width + threadIdx.x];
+            before += part_sh[1][i * width + threadIdx.x];
+        }
     place(a, mask, words, base_sh, scan_sh, t0, n, total, before);
 }
 
-// Tokens per CTA: one CTA up to 64 tokens, else about one chunk per SM; at most 1024 (the masks
-// are E * chunk / 8 bytes of shared memory).
+// Tokens per CTA: one CTA up to 32 tokens, else two CTAs an SM with a token a warp at least; at most 1024
+// (the masks are E * chunk / 8 bytes of shared memory).
 static int chunk_of(int T) {
-    if (T <= 64) return 64;
-    const int per = (T + num_sms() - 1) / num_sms();
-    const int c = (per + 31) / 32 * 32;
-    return c < 32 ? 32 : c > 1024 ? 1024 : c;
+    if (T <= 32) return 32;
+    const int per = (T + 2 * num_sms() - 1) / (2 * num_sms());
+    return per < kWarps ? kWarps : per > 1024 ? 1024 : per;
 }
 
-template <typename KeyT>
+static int experts_per_lane(int E) { return E <= 32 ? 1 : E <= 64 ? 2 : E <= 128 ? 4 : E <= 256 ? 8 : 16; }
+
 static cudaError_t launch_route(const RouteArgs &a, int chunks, size_t smem, cudaStream_t st) {
-    auto kern = a.E <= 32    ? route_kernel<1, KeyT>
-                : a.E <= 64  ? route_kernel<2, KeyT>
-                : a.E <= 128 ? route_kernel<4, KeyT>
-                : a.E <= 256 ? route_kernel<8, KeyT>
-                             : route_kernel<16, KeyT>;
-    if (smem > 40960) {  // above the default limit less the static arrays
+    void (*kern)(RouteArgs) = nullptr;
+    switch (experts_per_lane(a.E)) {
+        case 1: kern = route_kernel<1>; break;
+        case 2: kern = route_kernel<2>; break;
+        case 4: kern = route_kernel<4>; break;
+        case 8: kern = route_kernel<8>; break;
+        default: kern = route_kernel<16>;
+    }
+    if (smem > 32768) {  // above the default limit less the static arrays
         const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
     }
@@ -441,7 +768,8 @@ static int combine_out(const void *y, int rows, const int *slots, const float *w
 
 size_t moe_route_workspace(int T, int E) {
     const int c = moe::chunk_of(T);
-    return T <= c ? 0 : ((size_t)((T + c - 1) / c) * E * 4 + 255) & ~size_t(255);
+    const size_t chunks = (T + c - 1) / c;
+    return T <= c ? 0 : ((chunks + 7) / 8 * 8 * E * 2 + 255) & ~size_t(255);
 }
 
 int moe_route(const void *logits, int dtype, const float *bias, int T, int E, int k, int score, int groups,
@@ -467,13 +795,17 @@ int moe_route(const void *logits, int dtype, const float *bias, int T, int E, in
     a.rows = rows;
     a.slots = slots;
     a.chunk = chunk_of(T);
+    a.words = (a.chunk + 31) / 32;
     const int chunks = T > a.chunk ? (T + a.chunk - 1) / a.chunk : 1;
-    a.counts = chunks > 1 && offsets ? static_cast<int *>(workspace) : nullptr;
-    const size_t masks = offsets ? (size_t)E * (a.chunk / 32) * 4 : 0;
-    const size_t smem = ((masks + 15) & ~size_t(15)) + (groups > 1 ? (size_t)kWarps * E * 8 : 0);
-    // 64-bit keys where scores are compared, not logits
-    const bool wide = bias || (groups > 1 && a.top2);
-    W4_CUDA_TRY(wide ? launch_route<uint64_t>(a, chunks, smem, st) : launch_route<uint32_t>(a, chunks, smem, st));
+    a.counts = chunks > 1 && offsets ? static_cast<uint16_t *>(workspace) : nullptr;
+    const int epl = experts_per_lane(E), es = dtype == W4_F32 ? 4 : 2, width = epl * es < 16 ? epl * es : 16;
+    a.vec = E % epl == 0 && E * es % width == 0 && aligned(logits, width);
+    const int size = E / groups, lanes = size / epl;
+    a.whole = size % epl == 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
+    a.vec_bias = E % epl == 0 && aligned(bias, epl * 4 < 16 ? epl * 4 : 16);
+    const size_t masks = offsets ? (size_t)E * a.words * 4 : 0;
+    const size_t smem = ((masks + 15) & ~size_t(15)) + (groups > 1 && !a.whole ? (size_t)kWarps * (E + E / 32) * 8 : 0);
+    W4_CUDA_TRY(launch_route(a, chunks, smem, st));
     if (a.counts) {
         if (masks > 40960)
             W4_CUDA_TRY(cudaFuncSetAttribute(place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)masks));
