@@ -21,12 +21,11 @@ namespace moe {
 // tell apart: the choice would depend on how exp was rounded.  So a token is first chosen for in 32
 // bits, with one rank more than asked for, and where two neighbours (or the last group kept and the
 // next) are closer than the 32-bit errors, it is chosen for again in 64 (under 1 % of the tokens; all
-// in 64 bits took 61 us for 8192 x 256, top 8 of 4 in 8 groups, where this takes FIGURE).
+// in 64 bits took 61 us for 8192 x 256, top 8 of 4 in 8 groups, where this takes 25).
 //
 // The order by expert is a counting sort without atomics whose order matters: a token takes an
 // expert at most once, so a bit mask over a chunk's tokens for each expert gives counts (popc) and
 // ranks (popc below the token's bit).
-constexpr int kThreads = 512, kWarps = kThreads / 32;
 
 struct RouteArgs {
     const void *logits;
@@ -483,6 +482,7 @@ __device__ __forceinline__ void route_token(const RouteArgs &a, int t, const flo
 }
 
 // Exclusive prefix sum of v over the CTA's threads; the last one's inclusive sum in *total.
+template <int KT>
 __device__ __forceinline__ int block_scan(int v, int *sh, int *total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int inc = v;
@@ -494,7 +494,7 @@ __device__ __forceinline__ int block_scan(int v, int *sh, int *total) {
     if (lane == 31) sh[warp] = inc;
     __syncthreads();
     int before = 0, all = 0;
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < KT / 32; ++w) {
         const int u = sh[w];
         if (w < warp) before += u;
         all += u;
@@ -506,17 +506,18 @@ __device__ __forceinline__ int block_scan(int v, int *sh, int *total) {
 
 // Offsets, rows and slots of one chunk from its masks, the experts' totals and the counts of the
 // chunks before it (thread e: expert e).
+template <int KT>
 __device__ __forceinline__ void place(const RouteArgs &a, const uint32_t *mask, int words, int *base, int *sh, int t0,
                                       int n, int total, int before) {
     int all = 0;
-    const int start = block_scan(total, sh, &all);
+    const int start = block_scan<KT>(total, sh, &all);
     if ((int)threadIdx.x < a.E) {
         base[threadIdx.x] = start + before;
         if (blockIdx.x == 0) a.offsets[threadIdx.x] = start;
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) a.offsets[a.E] = all;
     __syncthreads();
-    for (int i = threadIdx.x; i < n * a.k; i += kThreads) {
+    for (int i = threadIdx.x; i < n * a.k; i += KT) {
         const int tl = i / a.k;
         const size_t o = (size_t)t0 * a.k + i;
         const int e = a.ids[o];
@@ -530,15 +531,15 @@ __device__ __forceinline__ void place(const RouteArgs &a, const uint32_t *mask, 
         a.slots[o] = pos;
     }
     const long end = (long)a.T * a.k;  // rows behind the last expert's
-    for (long i = (long)all + (long)blockIdx.x * kThreads + threadIdx.x; i < end; i += (long)gridDim.x * kThreads)
+    for (long i = (long)all + (long)blockIdx.x * KT + threadIdx.x; i < end; i += (long)gridDim.x * KT)
         a.rows[i] = -1;
 }
 
-template <int EPL>
-__global__ void __launch_bounds__(kThreads, EPL == 16 ? 1 : 2) route_kernel(const RouteArgs a) {
+template <int EPL, int KT>
+__global__ void __launch_bounds__(KT) route_kernel(const RouteArgs a) {
     extern __shared__ __align__(16) uint8_t sm[];
-    __shared__ int base_sh[kMaxMoeExperts], scan_sh[kWarps];
-    __shared__ __align__(16) Pick pick_sh[kWarps];
+    __shared__ int base_sh[kMaxMoeExperts], scan_sh[(KT / 32)];
+    __shared__ __align__(16) Pick pick_sh[(KT / 32)];
     const int words = a.words;
     uint32_t *mask = reinterpret_cast<uint32_t *>(sm);
     double *base = reinterpret_cast<double *>(sm + (((size_t)(a.offsets ? a.E * words : 0) * 4 + 15) & ~size_t(15))) +
@@ -547,17 +548,17 @@ __global__ void __launch_bounds__(kThreads, EPL == 16 ? 1 : 2) route_kernel(cons
     while (lpg * a.groups > 32) lpg >>= 1;
     grid_dep_launch();
     if (a.offsets)
-        for (int i = threadIdx.x; i < a.E * words; i += kThreads) mask[i] = 0;
+        for (int i = threadIdx.x; i < a.E * words; i += KT) mask[i] = 0;
     __syncthreads();
     grid_dep_wait();
     const int t0 = blockIdx.x * a.chunk, n = min(a.chunk, a.T - t0);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     float l[EPL], ahead[EPL];  // a token's logits are on their way while the one before it is chosen for
     if (warp < n) load_logits<EPL>(a, t0 + warp, lane, ahead);
-    for (int i = warp; i < n; i += kWarps) {
+    for (int i = warp; i < n; i += (KT / 32)) {
 #pragma unroll
         for (int u = 0; u < EPL; ++u) l[u] = ahead[u];
-        if (i + kWarps < n) load_logits<EPL>(a, t0 + i + kWarps, lane, ahead);
+        if (i + (KT / 32) < n) load_logits<EPL>(a, t0 + i + (KT / 32), lane, ahead);
         route_token<EPL>(a, t0 + i, l, base, lpg, &pick_sh[warp], mask, words, i);
     }
     if (!a.offsets) return;
@@ -574,43 +575,47 @@ __global__ void __launch_bounds__(kThreads, EPL == 16 ? 1 : 2) route_kernel(cons
                 for (int c = gridDim.x; c < pitch; ++c) col[c] = 0;
         }
     } else {
-        place(a, mask, words, base_sh, scan_sh, t0, n, count, 0);
+        place<KT>(a, mask, words, base_sh, scan_sh, t0, n, count, 0);
     }
 }
 
-__global__ void __launch_bounds__(kThreads) place_kernel(const RouteArgs a) {
+template <int KT>
+__global__ void __launch_bounds__(KT) place_kernel(const RouteArgs a) {
     extern __shared__ __align__(16) uint8_t sm[];
-    __shared__ int base_sh[kMaxMoeExperts], scan_sh[kWarps];
+    __shared__ int base_sh[kMaxMoeExperts], scan_sh[(KT / 32)];
     const int words = a.words;
     uint32_t *mask = reinterpret_cast<uint32_t *>(sm);
     grid_dep_launch();
-    for (int i = threadIdx.x; i < a.E * words; i += kThreads) mask[i] = 0;
+    for (int i = threadIdx.x; i < a.E * words; i += KT) mask[i] = 0;
     __syncthreads();
     grid_dep_wait();
     const int t0 = blockIdx.x * a.chunk, n = min(a.chunk, a.T - t0);
-    for (int i = threadIdx.x; i < n * a.k; i += kThreads) {
+    for (int i = threadIdx.x; i < n * a.k; i += KT) {
         const int e = a.ids[(size_t)t0 * a.k + i], tl = i / a.k;
         if (e >= 0) atomicOr(&mask[e * words + (tl >> 5)], 1u << (tl & 31));
     }
     // every chunk's counts, eight in 16 bytes: P threads an expert, then one
-    __shared__ int part_sh[2][kThreads];
+    __shared__ int part_sh[2][KT];
     int width = 32;
-    while (width < a.E) width <<= 1;  // at most kThreads
-    const int P = kThreads / width, e = threadIdx.x % width, c8 = (gridDim.x + 7) / 8;
+    while (width < a.E) width <<= 1;  // at most KT
+    const int P = KT / width, e = threadIdx.x % width, c8 = (gridDim.x + 7) / 8;
     unsigned total = 0, before = 0;
     if (e < a.E) {
         const uint4 *col = reinterpret_cast<const uint4 *>(a.counts) + (size_t)e * c8;
+        const int part = threadIdx.x / width, mine = blockIdx.x / 8;  // mine: the eight that hold this chunk
 #pragma unroll 8
-        for (int i = threadIdx.x / width; i < c8; i += P) {
+        for (int i = part; i < c8; i += P) {
             const uint4 v = col[i];
+            total = __dp2a_lo(v.w, 0x0101u, __dp2a_lo(v.z, 0x0101u, __dp2a_lo(v.y, 0x0101u, __dp2a_lo(v.x, 0x0101u, total))));
+            if (i < mine) before = total;
+        }
+        if (mine % P == part) {
+            const uint4 v = col[mine];
             const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            const int in = blockIdx.x % 8;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int c = 8 * i + 2 * u;  // chunks c and c + 1
-                total = __dp2a_lo(w[u], 0x0101u, total);
-                before = __dp2a_lo(w[u], (c < (int)blockIdx.x ? 1u : 0u) | (c + 1 < (int)blockIdx.x ? 0x100u : 0u),
-                                   before);
-            }
+            for (int u = 0; u < 4; ++u)
+                before = __dp2a_lo(w[u], (2 * u < in ? 1u : 0u) | (2 * u + 1 < in ? 0x100u : 0u), before);
         }
     }
     part_sh[0][threadIdx.x] = total;
@@ -622,33 +627,44 @@ __global__ void __launch_bounds__(kThreads) place_kernel(const RouteArgs a) {
             total += part_sh[0][i * width + threadIdx.x];
             before += part_sh[1][i * width + threadIdx.x];
         }
-    place(a, mask, words, base_sh, scan_sh, t0, n, total, before);
+    place<KT>(a, mask, words, base_sh, scan_sh, t0, n, total, before);
 }
 
-// Tokens per CTA: one CTA up to 32 tokens, else two CTAs an SM with a token a warp at least; at most 1024
-// (the masks are E * chunk / 8 bytes of shared memory).
-static int chunk_of(int T) {
-    if (T <= 32) return 32;
-    const int per = (T + 2 * num_sms() - 1) / (2 * num_sms());
-    return per < kWarps ? kWarps : per > 1024 ? 1024 : per;
+// Threads and tokens of a CTA.  Up to 32 tokens one CTA does everything.  Up to 16 an SM: 16 warps, a token
+// each (148 tokens: 8.4 us, with 32 warps 11.6).  More: one CTA of 32 warps an SM (8192 tokens: 25 us, with
+// two of 16 warps 28, since every CTA of the second kernel reads all counts); at most 1024 tokens (the
+// masks are E * chunk / 8 bytes of shared memory).
+struct Shape {
+    int threads, chunk;
+};
+static Shape shape_of(int T, int E) {
+    if (T <= 32) return {512, 32};
+    const int per = (T + num_sms() - 1) / num_sms();
+    if (per <= 16) return {512, 16};
+    return {E > 256 ? 512 : 1024, per > 1024 ? 1024 : per};  // 16 experts a lane take the registers of 512
 }
 
 static int experts_per_lane(int E) { return E <= 32 ? 1 : E <= 64 ? 2 : E <= 128 ? 4 : E <= 256 ? 8 : 16; }
 
-static cudaError_t launch_route(const RouteArgs &a, int chunks, size_t smem, cudaStream_t st) {
+template <int KT>
+static cudaError_t launch_route(const RouteArgs &a, int chunks, size_t masks, size_t smem, cudaStream_t st) {
     void (*kern)(RouteArgs) = nullptr;
     switch (experts_per_lane(a.E)) {
-        case 1: kern = route_kernel<1>; break;
-        case 2: kern = route_kernel<2>; break;
-        case 4: kern = route_kernel<4>; break;
-        case 8: kern = route_kernel<8>; break;
-        default: kern = route_kernel<16>;
+        case 1: kern = route_kernel<1, KT>; break;
+        case 2: kern = route_kernel<2, KT>; break;
+        case 4: kern = route_kernel<4, KT>; break;
+        case 8: kern = route_kernel<8, KT>; break;
+        default: kern = route_kernel<16, 512>;
     }
-    if (smem > 32768) {  // above the default limit less the static arrays
+    if (smem > 16384) {  // above the default limit less the static arrays
         const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
     }
-    return launch_decode(kern, dim3(chunks), dim3(kThreads), smem, st, 1, a);
+    cudaError_t e = launch_decode(kern, dim3(chunks), dim3(KT), smem, st, 1, a);
+    if (e != cudaSuccess || !a.counts) return e;
+    if (masks > 32768)
+        e = cudaFuncSetAttribute(place_kernel<KT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)masks);
+    return e != cudaSuccess ? e : launch_decode(place_kernel<KT>, dim3(chunks), dim3(KT), masks, st, 1, a);
 }
 
 // ---------------------------------------------------------------------------- combine
@@ -767,7 +783,7 @@ static int combine_out(const void *y, int rows, const int *slots, const float *w
 }  // namespace moe
 
 size_t moe_route_workspace(int T, int E) {
-    const int c = moe::chunk_of(T);
+    const int c = moe::shape_of(T, E).chunk;
     const size_t chunks = (T + c - 1) / c;
     return T <= c ? 0 : ((chunks + 7) / 8 * 8 * E * 2 + 255) & ~size_t(255);
 }
@@ -794,7 +810,8 @@ int moe_route(const void *logits, int dtype, const float *bias, int T, int E, in
     a.offsets = offsets;
     a.rows = rows;
     a.slots = slots;
-    a.chunk = chunk_of(T);
+    const Shape sh = shape_of(T, E);
+    a.chunk = sh.chunk;
     a.words = (a.chunk + 31) / 32;
     const int chunks = T > a.chunk ? (T + a.chunk - 1) / a.chunk : 1;
     a.counts = chunks > 1 && offsets ? static_cast<uint16_t *>(workspace) : nullptr;
@@ -804,13 +821,10 @@ int moe_route(const void *logits, int dtype, const float *bias, int T, int E, in
     a.whole = size % epl == 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
     a.vec_bias = E % epl == 0 && aligned(bias, epl * 4 < 16 ? epl * 4 : 16);
     const size_t masks = offsets ? (size_t)E * a.words * 4 : 0;
-    const size_t smem = ((masks + 15) & ~size_t(15)) + (groups > 1 && !a.whole ? (size_t)kWarps * (E + E / 32) * 8 : 0);
-    W4_CUDA_TRY(launch_route(a, chunks, smem, st));
-    if (a.counts) {
-        if (masks > 40960)
-            W4_CUDA_TRY(cudaFuncSetAttribute(place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)masks));
-        W4_CUDA_TRY(launch_decode(place_kernel, dim3(chunks), dim3(kThreads), masks, st, 1, a));
-    }
+    const size_t smem = ((masks + 15) & ~size_t(15)) +
+                        (groups > 1 && !a.whole ? (size_t)(sh.threads / 32) * (E + E / 32) * 8 : 0);
+    W4_CUDA_TRY(sh.threads == 1024 ? launch_route<1024>(a, chunks, masks, smem, st)
+                                   : launch_route<512>(a, chunks, masks, smem, st));
     return W4_OK;
 }
 
