@@ -330,6 +330,53 @@ __device__ __forceinline__ void store_cols(const Args &a, const uint32_t (&v)[LD
     }
 }
 
+// This CTA's share of a split tile's rows: the sums of the ks CTAs (KS, where it is known) added up, a warp
+// a row, four channels a lane, four rows in flight.
+template <bool PAIR, int KS>
+__device__ __forceinline__ void finish_split(const Args &a, const Tile &tl, const uint8_t *sm, const float *as_sh,
+                                             const float (&ws)[4], const float (&bs)[4], int rank, int kr, int ks) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const int n = tl.n0 + rank * BN + 4 * lane, r1 = tl.rows * (kr + 1) / ks;
+    for (int r0 = tl.rows * kr / ks + warp; r0 < r1; r0 += 4 * warps) {
+        int v[4][4] = {};
+        const int zs = KS ? KS : ks;
+#pragma unroll(KS ? KS : 2)
+        for (int z = 0; z < zs; ++z)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = min(r0 + i * warps, r1 - 1);
+                const uint8_t *at = sm + (row * BN + 4 * lane) * 4;
+                const int4 p = z == kr ? *reinterpret_cast<const int4 *>(at)
+                                       : ld_cluster_v4(at, PAIR ? 2 * z + rank : z);
+                v[i][0] += p.x;
+                v[i][1] += p.y;
+                v[i][2] += p.z;
+                v[i][3] += p.w;
+            }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = r0 + i * warps;
+            if (row >= r1 || n >= a.N) continue;
+            const float as = as_sh[row];
+            float y[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) y[u] = fmaf((float)v[i][u] * as, ws[u], bs[u]);
+            const size_t o = (size_t)(tl.row0 + row) * a.N + n;
+            if (a.wide && a.c_dtype == W4_BF16) {
+                *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.c) + o) =
+                    make_uint2(pack2<__nv_bfloat16>(y[0], y[1]), pack2<__nv_bfloat16>(y[2], y[3]));
+            } else if (a.wide && a.c_dtype == W4_F16) {
+                *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.c) + o) =
+                    make_uint2(pack2<__half>(y[0], y[1]), pack2<__half>(y[2], y[3]));
+            } else {
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (n + u < a.N) store_c(a, o + u, y[u]);
+            }
+        }
+    }
+}
+
 template <int BT, int MODE, bool PAIR>
 __global__ void __launch_bounds__(threads_of(BT, MODE), 1)
 s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap a_map, const Args a) {
@@ -593,67 +640,36 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
             }
         }
     }
+    // What the end of a split tile needs, on its way while the others finish.
+    float ws[4] = {}, bs[4] = {};
+    Tile last = {};
+    if (ks > 1 && t0 < ntiles) {
+        last = tile_of<MODE, PAIR>(a, t0, first, off);
+        const int n = last.n0 + rank * BN + 4 * lane;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (n + u < a.N) ws[u] = a.w_scale[(size_t)last.e * a.N + n + u];
+            if (n + u < a.N && a.bias) bs[u] = a.bias[(size_t)last.e * a.N + n + u];
+        }
+    }
     tc_fence_before();
     __syncthreads();
-    if constexpr (PAIR) cluster_sync_all();  // both CTAs are done with TMEM and each other's barriers
+    // a pair is done with its TMEM and each other's barriers; the CTAs of a split have stored their sums
+    if (PAIR || ks > 1) cluster_sync_all();
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc<PAIR>(tmem, C_::TMEM_COLS);
     }
-    if constexpr (PAIR) cluster_sync_all();
-    if (ks > 1) {
-        // The CTAs along z hold their parts of one tile's sums (s32: the order does not matter) where
-        // their stages were; each finishes an equal share of the rows, a warp a row, four channels a
-        // lane, four rows in flight.
-        cluster_sync_all();
-        if (t0 < ntiles) {
-            const Tile tl = tile_of<MODE, PAIR>(a, t0, first, off);
-            const int n = tl.n0 + rank * BN + 4 * lane, warps = blockDim.x >> 5;
-            float ws[4], bs[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                ws[u] = n + u < a.N ? a.w_scale[(size_t)tl.e * a.N + n + u] : 0.f;
-                bs[u] = n + u < a.N && a.bias ? a.bias[(size_t)tl.e * a.N + n + u] : 0.f;
-            }
-            const int r1 = tl.rows * (kr + 1) / ks;
-            for (int r0 = tl.rows * kr / ks + warp; r0 < r1; r0 += 4 * warps) {
-                int v[4][4] = {};
-#pragma unroll 4
-                for (int z = 0; z < ks; ++z)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int row = min(r0 + i * warps, r1 - 1);
-                        const int4 p = ld_cluster_v4(sm + (row * BN + 4 * lane) * 4, PAIR ? 2 * z + rank : z);
-                        v[i][0] += p.x;
-                        v[i][1] += p.y;
-                        v[i][2] += p.z;
-                        v[i][3] += p.w;
-                    }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int row = r0 + i * warps;
-                    if (row >= r1 || n >= a.N) continue;
-                    const float as = as_sh[row];
-                    float y[4];
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) y[u] = fmaf((float)v[i][u] * as, ws[u], bs[u]);
-                    const size_t o = (size_t)(tl.row0 + row) * a.N + n;
-                    if (a.wide && a.c_dtype == W4_BF16) {
-                        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.c) + o) =
-                            make_uint2(pack2<__nv_bfloat16>(y[0], y[1]), pack2<__nv_bfloat16>(y[2], y[3]));
-                    } else if (a.wide && a.c_dtype == W4_F16) {
-                        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.c) + o) =
-                            make_uint2(pack2<__half>(y[0], y[1]), pack2<__half>(y[2], y[3]));
-                    } else {
-#pragma unroll
-                        for (int u = 0; u < 4; ++u)
-                            if (n + u < a.N) store_c(a, o + u, y[u]);
-                    }
-                }
-            }
-        }
-        cluster_sync_all();  // nobody leaves while its sums are read
+    // The CTAs along z hold their parts of one tile's sums (s32: the order does not matter) where their
+    // stages were; each finishes an equal share of the rows.
+    switch (ks) {
+        case 1: break;
+        case 2: finish_split<PAIR, 2>(a, last, sm, as_sh, ws, bs, rank, kr, ks); break;
+        case 3: finish_split<PAIR, 3>(a, last, sm, as_sh, ws, bs, rank, kr, ks); break;
+        case 4: finish_split<PAIR, 4>(a, last, sm, as_sh, ws, bs, rank, kr, ks); break;
+        default: finish_split<PAIR, 0>(a, last, sm, as_sh, ws, bs, rank, kr, ks);
     }
+    if (PAIR || ks > 1) cluster_sync_all();  // nobody leaves while its sums are read
 }
 
 template <int BT, int MODE, bool PAIR = false>

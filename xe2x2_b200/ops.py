@@ -573,9 +573,9 @@ def moe_route(logits, top_k, bias=None, score="softmax", renormalize=True, scali
     if top_k < 1:
         raise ValueError(f"top_k must be at least 1, got {top_k}")
     i32 = torch.int32
-    ids, weights = logits.new_empty((T, top_k), dtype=i32), logits.new_empty((T, top_k), dtype=torch.float32)
+    ids = logits.new_empty((T, top_k), dtype=i32)
+    weights, slots = torch.empty_like(ids, dtype=torch.float32), torch.empty_like(ids)
     offsets, rows = logits.new_empty(E + 1, dtype=i32), logits.new_empty(T * top_k, dtype=i32)
-    slots = logits.new_empty((T, top_k), dtype=i32)
     need = L.lib().w4_moe_route_workspace_bytes(T, E)
     ws = logits.new_empty(need, dtype=torch.uint8) if need else None
     _call_on(dev, "w4_moe_route", pl, _FLOATS[logits.dtype], pb, T, E, top_k, _SCORES[score], int(n_group),
