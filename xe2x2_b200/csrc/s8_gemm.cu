@@ -45,12 +45,9 @@ struct Args {
     int c_dtype, M, a_rows, N, K, E;
     int bt, box;  // token rows of a tile (a multiple of 16), of one token copy
     int ntn;      // column tiles
-    bool wide;    // 16-bit rows of C can be stored 16 bytes at a time (N % 8 == 0, c 16-byte aligned)
+    bool pairs;   // 16-bit rows of C can be stored four bytes at a time (N even, c aligned)
+    bool wide;    // and eight
 };
-
-// The epilogue's transposition buffer of a warp: 16 token pairs x 32 channels of 32 bits, rows
-// 36 words apart so that both the writes and the 16-byte reads touch every bank once.
-constexpr int TR_ROW = 36, TR_WORDS = 16 * TR_ROW;
 
 // BT token rows at most, S stages, two accumulators of BT columns.  PAIR: two CTAs (a cluster) on one
 // tile of 256 channels; each holds its 128 channels and half of the token rows.
@@ -60,8 +57,7 @@ template <int BT, bool PAIR> struct Cfg {
     static constexpr int S = STAGE > 40960 ? 4 : STAGE > 28672 ? 6 : STAGE > 20480 ? 8 : 5;
     static constexpr uint32_t TMEM_COLS = 2 * BT < 32 ? 32 : 2 * BT;
     static constexpr uint32_t BAR_OFF = S * STAGE, AS_OFF = BAR_OFF + (2 * S + 5) * 8 / 16 * 16 + 16,
-                              TR_OFF = AS_OFF + 2 * BT * 4, MISC_OFF = TR_OFF + EPI * TR_WORDS * 4,
-                              TILE_OFF = MISC_OFF + 16;
+                              MISC_OFF = AS_OFF + 2 * BT * 4, TILE_OFF = MISC_OFF + 16;
     static constexpr uint32_t LD = BT < 32 ? BT : 32;  // columns of one TMEM read
     static constexpr size_t smem(int E) { return TILE_OFF + (size_t)2 * (E + 1) * 4 + 1024; }
     static_assert(TILE_OFF + 2 * (kMaxMoeExperts + 1) * 4 + 1024 <= 227 * 1024, "shared memory plan");
@@ -267,37 +263,30 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     }
 }
 
-// LD token columns of a warp's 32 channels, as 16-bit rows of C: pairs of tokens go through shared
-// memory word by word and come back as eight channels of one token, 16 bytes a store.
+// LD token columns of a warp's 32 channels, as 16-bit rows of C: neighbouring lanes exchange a pair of
+// tokens, and each stores two channels of one of them (4 bytes, 64 in a row to a half warp).  Through
+// shared memory, 16 bytes a store, the epilogue took a share of the bandwidth that the copies and the
+// MMAs use up (128 bytes a cycle at 256 x 256): M = 24,576, K = 2688, N = 3712
+// 178 -> 182 us, K = 1024 114 -> 96.
 template <int LD, typename T>
 __device__ __forceinline__ void store_rows(const Args &a, const uint32_t (&v)[LD], const float *as, float ws, float bs,
-                                           uint32_t *tr, int row, int rows, int n, int lane) {
+                                           int row, int rows, int n, int lane) {
+    const int odd = lane & 1;
+    const uint32_t sel = odd ? 0x3276u : 0x5410u;
+    T *dst = static_cast<T *>(a.c) + (size_t)(row + odd) * a.N + (n & ~1);
+    const bool in = n < a.N;  // N is even
 #pragma unroll
     for (int i = 0; i < LD / 4; ++i) {
         const float4 s = *reinterpret_cast<const float4 *>(as + 4 * i);
-        tr[2 * i * TR_ROW + lane] = pack2<T>(fmaf((float)(int)v[4 * i] * s.x, ws, bs),
-                                             fmaf((float)(int)v[4 * i + 1] * s.y, ws, bs));
-        tr[(2 * i + 1) * TR_ROW + lane] = pack2<T>(fmaf((float)(int)v[4 * i + 2] * s.z, ws, bs),
-                                                   fmaf((float)(int)v[4 * i + 3] * s.w, ws, bs));
+        const uint32_t p = pack2<T>(fmaf((float)(int)v[4 * i] * s.x, ws, bs), fmaf((float)(int)v[4 * i + 1] * s.y, ws, bs));
+        const uint32_t q =
+            pack2<T>(fmaf((float)(int)v[4 * i + 2] * s.z, ws, bs), fmaf((float)(int)v[4 * i + 3] * s.w, ws, bs));
+        const uint32_t w0 = __byte_perm(p, __shfl_xor_sync(0xffffffffu, p, 1), sel);
+        const uint32_t w1 = __byte_perm(q, __shfl_xor_sync(0xffffffffu, q, 1), sel);
+        if (in && 4 * i + odd < rows) *reinterpret_cast<uint32_t *>(dst) = w0;
+        if (in && 4 * i + 2 + odd < rows) *reinterpret_cast<uint32_t *>(dst + 2 * (size_t)a.N) = w1;
+        dst += 4 * (size_t)a.N;
     }
-    __syncwarp();
-    const int seg = (lane & 3) * 8;  // channels n + seg .. n + seg + 7
-#pragma unroll
-    for (int h = 0; h < LD / 16; ++h) {
-        const int pair = (lane >> 2) + 8 * h;
-        const uint4 x = *reinterpret_cast<const uint4 *>(tr + pair * TR_ROW + seg);
-        const uint4 y = *reinterpret_cast<const uint4 *>(tr + pair * TR_ROW + seg + 4);
-        T *dst = static_cast<T *>(a.c) + (size_t)(row + 2 * pair) * a.N + n + seg;
-        if (n + seg < a.N && 2 * pair < rows)
-            *reinterpret_cast<uint4 *>(dst) =
-                make_uint4(__byte_perm(x.x, x.y, 0x5410), __byte_perm(x.z, x.w, 0x5410), __byte_perm(y.x, y.y, 0x5410),
-                           __byte_perm(y.z, y.w, 0x5410));
-        if (n + seg < a.N && 2 * pair + 1 < rows)
-            *reinterpret_cast<uint4 *>(dst + a.N) =
-                make_uint4(__byte_perm(x.x, x.y, 0x7632), __byte_perm(x.z, x.w, 0x7632), __byte_perm(y.x, y.y, 0x7632),
-                           __byte_perm(y.z, y.w, 0x7632));
-    }
-    __syncwarp();
 }
 
 // A gather warp's finished stage: every lane orders its copies into its own CTA's shared memory before
@@ -313,7 +302,7 @@ __device__ __forceinline__ void hand_over(uint64_t *bar, uint32_t lead, int lane
     }
 }
 
-// The same column by column, for rows that cannot be stored in 16 bytes (f32, odd N): a warp's 32
+// The same column by column, for rows that cannot be stored in pairs (f32, odd N): a warp's 32
 // channels of one token are one store.
 template <int LD, typename T>
 __device__ __forceinline__ void store_cols(const Args &a, const uint32_t (&v)[LD], const float *as, float ws, float bs,
@@ -549,6 +538,10 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
         // ---------------- gather: token rows through the index, 16 bytes a lane and copy ----------------
         // The warps take the stages in turn.  Lane (r, c) of four rows a copy: chunk c of row r lies at
         // c ^ (r % 8) of its 128-byte line.  Row numbers are spread over the lanes, 32 a register.
+        // S >= kGather: a warp that waits for stage g's last use to end knows that use g - kGather - S has
+        // ended, and the parity it waits for means the right phase only if use g - 2 S is no later.
+        // (Handing a stage over only after the next one's copies were issued: 314 us for 257.)
+        static_assert(S >= kGather, "stage parity");
         constexpr int ROWS = PAIR ? BT / 2 : BT;
         const int r0 = lane >> 3, c = lane & 7;
         int g = 0;
@@ -588,7 +581,6 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
     } else {
         // ---------------- epilogue: lane quarter warp % 4 ----------------
         const int q = warp & 3, ew = warp - 2;
-        uint32_t *tr = reinterpret_cast<uint32_t *>(sm + C_::TR_OFF) + ew * TR_WORDS;
         bool ok = true;
         int j = 0;
         for (int t = t0; t < ntiles; t += tstep, ++j) {
@@ -618,12 +610,10 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
                     int *red = reinterpret_cast<int *>(sm) + c0 * BN + 32 * q + lane;
 #pragma unroll
                     for (int i = 0; i < (int)C_::LD; ++i) red[i * BN] = (int)v[i];
-                } else if (a.wide && a.c_dtype == W4_BF16) {
-                    store_rows<C_::LD, __nv_bfloat16>(a, v, as + c0, ws, bs, tr, tl.row0 + c0, tl.rows - c0,
-                                                      n0 + 32 * q, lane);
-                } else if (a.wide && a.c_dtype == W4_F16) {
-                    store_rows<C_::LD, __half>(a, v, as + c0, ws, bs, tr, tl.row0 + c0, tl.rows - c0, n0 + 32 * q,
-                                               lane);
+                } else if (a.pairs && a.c_dtype == W4_BF16) {
+                    store_rows<C_::LD, __nv_bfloat16>(a, v, as + c0, ws, bs, tl.row0 + c0, tl.rows - c0, n, lane);
+                } else if (a.pairs && a.c_dtype == W4_F16) {
+                    store_rows<C_::LD, __half>(a, v, as + c0, ws, bs, tl.row0 + c0, tl.rows - c0, n, lane);
                 } else if (in) {
                     if (a.c_dtype == W4_F32)
                         store_cols<C_::LD, float>(a, v, as + c0, ws, bs, tl.row0 + c0, tl.rows - c0, n);
@@ -758,7 +748,7 @@ int s8_gemm(const int8_t *a, const float *a_scale, const int8_t *w, const float 
     using namespace s8g;
     const Plan p = plan_for(M, N, K);
     const Args g = {a, a_scale, w_scale, bias, nullptr, nullptr, c, c_dtype, M, M, N, K, 1, p.bt,
-                    p.pair ? p.bt / 2 : p.bt, p.ntn, N % 8 == 0 && aligned(c, 16)};
+                    p.pair ? p.bt / 2 : p.bt, p.ntn, N % 2 == 0 && aligned(c, 4), N % 4 == 0 && aligned(c, 8)};
     CUtensorMap w_map, a_map;
     if (!make_map_3d(&w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, w, K, N, 1, K, (uint64_t)N * K, BK, BN,
                      CU_TENSOR_MAP_SWIZZLE_128B) ||
@@ -778,7 +768,7 @@ int s8_gemm_grouped(const int8_t *a, int a_rows, const float *a_scale, const int
     const int BT = rows <= 16 ? 16 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
     const bool pair = BT == 256 && N > BN;
     const Args g = {a, a_scale, w_scale, bias, offsets, src, c, c_dtype, R, a_rows, N, K, E, BT, BT < 32 ? BT : 32,
-                    pair ? (N + 2 * BN - 1) / (2 * BN) : (N + BN - 1) / BN, N % 8 == 0 && aligned(c, 16)};
+                    pair ? (N + 2 * BN - 1) / (2 * BN) : (N + BN - 1) / BN, N % 2 == 0 && aligned(c, 4), N % 4 == 0 && aligned(c, 8)};
     CUtensorMap w_map, a_map;
     if (!make_map_3d(&w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, w, K, N, E, K, (uint64_t)N * K, BK, BN,
                      CU_TENSOR_MAP_SWIZZLE_128B) ||
