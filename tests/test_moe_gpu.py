@@ -274,3 +274,29 @@ def test_combine_ignores_what_no_slot_names(cuda):
     w[1, 0] = float("nan")  # a token whose logits were NaN stays visible
     assert torch.isnan(ops.moe_combine(y, slots, w)[1]).all()
     assert ops.moe_combine(y, slots[:0], w[:0]).shape == (0, 64)
+
+
+# ------------------------------------------------------------------------------------- many tokens
+@pytest.mark.parametrize("score,G,tg,group_score", [("sigmoid", 1, 1, "max"), ("sigmoid", 8, 4, "top2"),
+                                                    ("softmax", 1, 1, "max"), ("softmax", 8, 3, "max"),
+                                                    ("softmax", 4, 2, "top2")])
+@pytest.mark.parametrize("E", [256, 96])
+def test_every_choice_of_many_tokens_is_the_64_bit_one(cuda, E, score, G, tg, group_score):
+    """Among 200,000 tokens hundreds have neighbours that 32 bits cannot tell apart."""
+    T, k = 200_000, 8
+    x = _logits(T, E, "f32", E + G, cuda)
+    bias = 0.1 * torch.randn(E, device=cuda, generator=torch.Generator(device=cuda).manual_seed(7))
+    r = ops.moe_route(x, k, bias, score, n_group=G, topk_group=tg, group_score=group_score)
+    xd = x.double()
+    p = torch.softmax(xd, 1) if score == "softmax" else torch.sigmoid(xd)
+    key = p + bias.double()
+    if G > 1:
+        best = key.view(T, G, E // G).topk(2, dim=2).values
+        tot = best[:, :, 0] + (best[:, :, 1] if group_score == "top2" else 0)
+        kept = torch.zeros(T, G, dtype=torch.bool, device=cuda).scatter_(1, tot.topk(tg, dim=1).indices, True)
+        key = key.masked_fill(~kept.repeat_interleave(E // G, 1), -float("inf"))
+    ids = torch.sort(key, dim=1, descending=True, stable=True).indices[:, :k]
+    assert torch.equal(r.ids.long(), ids)
+    w = p.gather(1, ids)
+    w = w / w.sum(1, keepdim=True)
+    assert float(((r.weights.double() - w) / w).abs().max()) < 1e-5

@@ -21,7 +21,7 @@ namespace moe {
 // tell apart: the choice would depend on how exp was rounded.  So a token is first chosen for in 32
 // bits, with one rank more than asked for, and where two neighbours (or the last group kept and the
 // next) are closer than the 32-bit errors, it is chosen for again in 64 (under 1 % of the tokens; all
-// in 64 bits took 61 us for 8192 x 256, top 8 of 4 in 8 groups, where this takes 25).
+// in 64 bits took 61 us for 8192 x 256, top 8 of 4 in 8 groups, where this takes 21).
 //
 // The order by expert is a counting sort without atomics whose order matters: a token takes an
 // expert at most once, so a bit mask over a chunk's tokens for each expert gives counts (popc) and
@@ -204,9 +204,11 @@ struct Pick {
 
 // The kk <= 32 largest keys in order, the j-th to lane j (*m = 0 where there is none), in a fixed number
 // of steps: the kk-th largest of the lanes' maxima bounds the kk-th largest key from below, and the
-// few keys from there on are ranked against each other.  False if those are more than 32.
+// few keys from there on are ranked against each other (all *count of them, down to *from, are left in
+// order in p->out).  False if those are more than 32.
 template <int EPL>
-__device__ __forceinline__ bool select32(const uint32_t (&key)[EPL], int kk, int lane, Pick *p, int *e, uint32_t *m) {
+__device__ __forceinline__ bool select32(const uint32_t (&key)[EPL], int kk, int lane, Pick *p, int *e, uint32_t *m,
+                                         int *count, uint32_t *from) {
     uint32_t best = key[0];
 #pragma unroll
     for (int i = 1; i < EPL; ++i) best = max(best, key[i]);
@@ -229,6 +231,8 @@ __device__ __forceinline__ bool select32(const uint32_t (&key)[EPL], int kk, int
         n += __popc(b);
     }
     __syncwarp();
+    *count = n;
+    *from = least;
     if (n > 32) return false;
     const uint2 mine = lane < n ? p->cand[lane] : make_uint2(0u, 0u);
     int rank = 0;
@@ -342,12 +346,12 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const Token<EPL> &k, 
     }
     c->e = -1;
     KeyT mine = 0;  // lane j: the j-th key; in doubt also the one behind the last
-    uint32_t last = 0;
-    int last_e = -1;
+    uint32_t last = 0, from = 0;
+    int last_e = -1, n = 0;
     bool done = false;
     if constexpr (NARROW) {
         const int kk = a.k + (doubt && a.bias ? 1 : 0);
-        if (kk <= 32 && select32<EPL>(key, kk, lane, pick, &c->e, &mine)) {
+        if (kk <= 32 && select32<EPL>(key, kk, lane, pick, &c->e, &mine, &n, &from)) {
             done = true;
             last = __shfl_sync(0xffffffffu, mine, a.k & 31);
             last_e = __shfl_sync(0xffffffffu, c->e, a.k & 31);
@@ -382,7 +386,26 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const Token<EPL> &k, 
                 if (x - y <= close_to(a.softmax, fmaxf(x - bx, y - by), x))
                     near = bx != by || logit_of(a, k.t, c->e) != logit_of(a, k.t, e2);
             }
-            if (__any_sync(0xffffffffu, near)) return false;
+            if (__any_sync(0xffffffffu, near)) {
+                // A sigmoid needs no other expert: if every key that could reach the top_k is among those
+                // that were ranked, these are ranked again by score + bias in 64 bits, one a lane.
+                const uint32_t kth = __shfl_sync(0xffffffffu, mine, a.k - 1);
+                const float x = from_ordered(kth);
+                if (!done || a.softmax || (kth != 0 && x - from_ordered(from) <= 2 * close_to(false, 0.f, x))) return false;
+                const int e = lane < n ? (int)pick->out[lane].y : -1;
+                double v = -HUGE_VAL;
+                if (e >= 0) v = score_of(fminf(logit_of(a, k.t, e), FLT_MAX), false, 0.f, 0.0) + (double)a.bias[e];
+                int rank = 0;
+                for (int o = 0; o < n; ++o) {
+                    const double u = __shfl_sync(0xffffffffu, v, o);
+                    const int oe = __shfl_sync(0xffffffffu, e, o);
+                    rank += u > v || (u == v && oe < e);
+                }
+                if (lane < n) pick->cand[rank] = make_uint2(0u, e);
+                __syncwarp();
+                c->e = lane < n && lane < a.k ? (int)pick->cand[lane].y : -1;
+                __syncwarp();
+            }
         }
     }
     return true;
