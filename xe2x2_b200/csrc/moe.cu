@@ -21,7 +21,7 @@ namespace moe {
 // tell apart: the choice would depend on how exp was rounded.  So a token is first chosen for in 32
 // bits, with one rank more than asked for, and where two neighbours (or the last group kept and the
 // next) are closer than the 32-bit errors, it is chosen for again in 64 (under 1 % of the tokens; all
-// in 64 bits took 61 us for 8192 x 256, top 8 of 4 in 8 groups, where this takes 21).
+// in 64 bits took 61 us for 8192 x 256, top 8 of 4 in 8 groups, where this takes 20).
 //
 // The order by expert is a counting sort without atomics whose order matters: a token takes an
 // expert at most once, so a bit mask over a chunk's tokens for each expert gives counts (popc) and
@@ -36,7 +36,7 @@ struct RouteArgs {
     int *ids;
     float *weights;
     int *offsets, *rows, *slots;  // null: no plan
-    uint16_t *counts;             // [E][chunks, padded to 8 with zeros], null with one chunk
+    uint16_t *counts;             // [chunks / 8, rounded up][E][8], zeros behind the last; null with one chunk
     int chunk, words;             // tokens per CTA, and words of their bit masks
     bool vec, vec_bias;           // a lane's logits, its biases, are aligned to their size or 16
 };
@@ -590,12 +590,11 @@ __global__ void __launch_bounds__(KT) route_kernel(const RouteArgs a) {
     if ((int)threadIdx.x < a.E)
         for (int w = 0; w < words; ++w) count += __popc(mask[threadIdx.x * words + w]);
     if (a.counts) {
-        const int pitch = (gridDim.x + 7) / 8 * 8;
         if ((int)threadIdx.x < a.E) {
-            uint16_t *col = a.counts + (size_t)threadIdx.x * pitch;
-            col[blockIdx.x] = (uint16_t)count;  // at most 1024
+            uint16_t *eight = a.counts + ((size_t)(blockIdx.x / 8) * a.E + threadIdx.x) * 8;
+            eight[blockIdx.x % 8] = (uint16_t)count;  // at most 1024
             if (blockIdx.x == gridDim.x - 1)
-                for (int c = gridDim.x; c < pitch; ++c) col[c] = 0;
+                for (int c = blockIdx.x % 8 + 1; c < 8; ++c) eight[c] = 0;
         }
     } else {
         place<KT>(a, mask, words, base_sh, scan_sh, t0, n, count, 0);
@@ -624,16 +623,16 @@ __global__ void __launch_bounds__(KT) place_kernel(const RouteArgs a) {
     const int P = KT / width, e = threadIdx.x % width, c8 = (gridDim.x + 7) / 8;
     unsigned total = 0, before = 0;
     if (e < a.E) {
-        const uint4 *col = reinterpret_cast<const uint4 *>(a.counts) + (size_t)e * c8;
+        const uint4 *col = reinterpret_cast<const uint4 *>(a.counts) + e;  // neighbours in 16 bytes each
         const int part = threadIdx.x / width, mine = blockIdx.x / 8;  // mine: the eight that hold this chunk
 #pragma unroll 8
         for (int i = part; i < c8; i += P) {
-            const uint4 v = col[i];
+            const uint4 v = col[(size_t)i * a.E];
             total = __dp2a_lo(v.w, 0x0101u, __dp2a_lo(v.z, 0x0101u, __dp2a_lo(v.y, 0x0101u, __dp2a_lo(v.x, 0x0101u, total))));
             if (i < mine) before = total;
         }
         if (mine % P == part) {
-            const uint4 v = col[mine];
+            const uint4 v = col[(size_t)mine * a.E];
             const uint32_t w[4] = {v.x, v.y, v.z, v.w};
             const int in = blockIdx.x % 8;
 #pragma unroll
