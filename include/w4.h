@@ -15,7 +15,7 @@
  *     workspace is first used; every call that completes leaves it zero, so a
  *     workspace zeroed once stays usable for any later call.  After a call
  *     whose kernel reported W4_ERR_TIMEOUT (w4_check_device_status), zero it
- *     again.
+ *     again.  (w4_s8_gemm*, w4_moe_route: plain scratch instead, no sync area.)
  *   - Argument errors are reported synchronously (W4_ERR_INVALID /
  *     W4_ERR_UNSUPPORTED) before anything is launched; launch failures are
  *     W4_ERR_CUDA.  w4_last_error() gives a one-line reason (thread-local).
@@ -360,8 +360,9 @@ enum w4_quant_fn {
  * x f16 / bf16 / f32 (x_dtype) as listed at w4_quant_fn, q s8 [M, K], scale f32 [M].  y is held
  * in f32 and never rounded to x_dtype.  A row in which y has a NaN or an infinity gets that
  * as its scale and zero codes, so products with it are NaN.  The arithmetic is that of
- * w4_rmsnorm_quant_s8 without the norm (kernels/epilogue_quant/rmsnorm_epilogue.cpp:56-70).
- * K % 16 == 0, x and q 16-byte aligned, M >= 0. */
+ * w4_rmsnorm_quant_s8 without the norm (kernels/epilogue_quant/rmsnorm_epilogue.cpp:56-70); with
+ * W4_FN_SILU_MUL y is within about 1e-6 (relative) of the formula.
+ * K % 16 == 0, x and q 16-byte aligned and not overlapping, M >= 0. */
 int w4_quant_s8(const void *x, int x_dtype, int fn, int8_t *q, float *scale, int M, int K, void *stream);
 
 /* W8A8 GEMM:  C[m,n] = (sum_k a[m,k] * w[n,k]) * a_scale[m] * w_scale[n] + bias[n]
@@ -416,7 +417,8 @@ enum w4_moe_group_score {
  * An expert whose logit is -inf (or whose bias is -inf or NaN) is never chosen.  A token that has
  * fewer than top_k experts to choose from gets id -1 and weight 0 in the slots left over, so a row
  * of -inf (padding) goes nowhere.  A NaN logit counts as -inf for the choice, and every weight of
- * its token is NaN.  An infinite logit counts as the largest finite one.
+ * its token is NaN.  An infinite logit counts as the largest finite one in
+ * the scores.
  *
  * The order by expert (all three or none):
  *   offsets i32 [E + 1]:      expert e's rows are [offsets[e], offsets[e + 1]), ordered by token
