@@ -40,7 +40,7 @@ def _check(out, acc, a_scale, w_scale, bias):
 DENSE = [(1, 1, 16), (1, 128, 128), (2, 3, 32), (3, 130, 48), (16, 256, 2688), (17, 64, 1856), (33, 300, 144),
          (64, 512, 512), (65, 1000, 272), (100, 256, 1024), (128, 127, 640), (129, 129, 1040), (200, 333, 4096),
          (300, 2688, 1856), (1000, 384, 512), (257, 4224, 256), (5, 5120, 17408), (1, 5120, 5120), (2, 17408, 5120),
-         (700, 5120, 640), (2050, 1856, 2688)]
+         (700, 5120, 640), (2050, 1856, 2688), (3, 257, 4096), (40, 131, 8192), (150, 259, 4096), (250, 130, 2064)]
 
 
 @pytest.mark.parametrize("out", list(DTYPES))

@@ -29,8 +29,8 @@ namespace s8g {
 
 constexpr int BN = 128, BK = 128;  // output channels and bytes of K in a stage
 constexpr int kGather = 4;  // gather warps
-// Epilogue warps (from warp 2 on): two to a lane quarter for the widest tile.  16 bytes a store hardly
-// need the second one (M = 24,576, K = 2688, N = 3712, bf16: 175 and 181 us), f32 and odd N do (262 -> 215).
+// Epilogue warps (from warp 2 on): two to a lane quarter for the widest tile (M = 24,576, K = 2688,
+// N = 3712: f32 262 -> 215 us, bf16 within 4 %).
 constexpr int epi_warps(int bt) { return bt == 256 ? 8 : 4; }
 constexpr uint32_t W_BYTES = BN * BK;
 
@@ -266,8 +266,8 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 // LD token columns of a warp's 32 channels, as 16-bit rows of C: neighbouring lanes exchange a pair of
 // tokens, and each stores two channels of one of them (4 bytes, 64 in a row to a half warp).  Through
 // shared memory, 16 bytes a store, the epilogue took a share of the bandwidth that the copies and the
-// MMAs use up (128 bytes a cycle at 256 x 256): M = 24,576, K = 2688, N = 3712
-// 178 -> 182 us, K = 1024 114 -> 96.
+// MMAs use up (128 bytes a cycle at 256 x 256): M = 24,576, N = 3712 at K = 1024 took 114 us, not 96 (at
+// K = 2688 178 and 182).
 template <int LD, typename T>
 __device__ __forceinline__ void store_rows(const Args &a, const uint32_t (&v)[LD], const float *as, float ws, float bs,
                                            int row, int rows, int n, int lane) {
@@ -409,7 +409,6 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
         prefetch_tensormap(&a_map);
     }
     if (warp == 1) tmem_alloc<PAIR>(tmem_slot, C_::TMEM_COLS);
-    grid_dep_launch();
     grid_dep_wait();
     int ntiles;
     if constexpr (MODE == kDense) {
@@ -630,6 +629,9 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
             }
         }
     }
+    // Not before: the next grid's CTAs would take what slots are free, unevenly (M = 16, K = N = 5120: 8.9 us
+    // where this takes 7.6).
+    grid_dep_launch();
     // What the end of a split tile needs, on its way while the others finish.
     float ws[4] = {}, bs[4] = {};
     Tile last = {};
