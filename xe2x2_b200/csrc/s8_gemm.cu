@@ -664,6 +664,47 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
     if (PAIR || ks > 1) cluster_sync_all();  // nobody leaves while its sums are read
 }
 
+// Clusters of `cluster` CTAs of a kernel (shared memory set) that the current device runs at once; asked
+// of the runtime once a device.
+static int clusters_at_once(const void *kern, int threads, size_t smem, int pair, int ks, int *cache) {
+    if (*cache > 0) return *cache;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(pair ? 2 : 1, 1, ks);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = pair ? 2 : 1;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = ks;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
+        (void)cudaGetLastError();
+        n = num_sms() / (ks * (pair ? 2 : 1)) / 2;  // a careful guess
+    }
+    *cache = n > 0 ? n : 1;
+    return *cache;
+}
+// Of the dense kernels, by plan: tile c (16, 64, 128, 256, pair) and K split.
+static int dense_clusters(int c, int ks) {
+    static std::mutex mu;
+    static int cache[16][5][9] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 16) dev = 0;
+    std::lock_guard<std::mutex> lk(mu);
+    int *at = &cache[dev][c][ks];
+    switch (c) {
+        case 0: return clusters_at_once((const void *)s8_gemm_kernel<16, kDense, false>, threads_of(16, kDense), Cfg<16, false>::smem(0), 0, ks, at);
+        case 1: return clusters_at_once((const void *)s8_gemm_kernel<64, kDense, false>, threads_of(64, kDense), Cfg<64, false>::smem(0), 0, ks, at);
+        case 2: return clusters_at_once((const void *)s8_gemm_kernel<128, kDense, false>, threads_of(128, kDense), Cfg<128, false>::smem(0), 0, ks, at);
+        case 3: return clusters_at_once((const void *)s8_gemm_kernel<256, kDense, false>, threads_of(256, kDense), Cfg<256, false>::smem(0), 0, ks, at);
+        default: return clusters_at_once((const void *)s8_gemm_kernel<256, kDense, true>, threads_of(256, kDense), Cfg<256, true>::smem(0), 1, ks, at);
+    }
+}
+
 template <int BT, int MODE, bool PAIR = false>
 static int launch(const CUtensorMap &w_map, const CUtensorMap &a_map, const Args &a, int grid, int ks,
                   cudaStream_t st) {
@@ -704,10 +745,13 @@ struct Plan {
     long tiles;
 };
 
-// The plan with the least estimated cycles.  A k-block of 128 takes 2 bt tensor cycles, or longer to
-// arrive at 64 bytes a cycle and SM (128 channels and bt rows; a pair's CTA has half of the rows);
-// tiles go in waves over the SMs; a K split (a cluster of at most 8 CTAs, four k-blocks each at
-// least, one tile a cluster) costs an exchange; and nothing is faster than memory.
+// The plan with the least estimated cycles, from measured times of the plans on some 30 shapes of 1 to
+// 8192 tokens.  A k-block of 128 takes 2 bt tensor cycles, or longer to arrive (128 channels and bt rows
+// at 58 bytes a cycle and SM; a pair's CTA has half of the rows and gets 64), and 500 at least; tiles go
+// in waves over the SMs; a pair costs 4500 for its barriers and fill; a K split (a cluster of at most 8
+// CTAs, four k-blocks each at least, one tile a cluster, all clusters at once) costs its exchange; and
+// nothing is faster than memory.  Within 2 % of the best of all plans on most of the shapes, 15 % off at worst
+// (150 x 4096 x 1024).
 static Plan plan_for(int M, int N, int K) {
     const int nsm = num_sms(), nkb = (K + BK - 1) / BK;
     Plan best = {};
@@ -723,12 +767,14 @@ static Plan plan_for(int M, int N, int K) {
         p.ntn = p.pair ? (N + 2 * BN - 1) / (2 * BN) : (N + BN - 1) / BN;
         p.tiles = (long)((M + p.bt - 1) / p.bt) * p.ntn;
         const int slots = p.pair ? nsm / 2 : nsm;
-        const double per_kb = p.pair ? (256 + p.bt > 2 * p.bt ? 256 + p.bt : 2 * p.bt) : 256 + 2 * p.bt;
+        double per_kb = p.pair ? (256 + p.bt > 2 * p.bt ? 256 + p.bt : 2 * p.bt) : 1.1 * (256 + 2 * p.bt);
+        per_kb = per_kb > 500 ? per_kb : 500;
         for (p.ks = 1; p.ks <= (p.pair ? 4 : 8); ++p.ks) {
-            if (p.ks > 1 && (p.tiles * p.ks > slots || nkb / p.ks < 4)) break;
-            const double waves = (double)((p.tiles * p.ks + slots - 1) / slots);
+            if (p.ks > 1 && (p.tiles * p.ks > slots || nkb / p.ks < 4 || p.tiles > dense_clusters(c, p.ks))) break;
+            const double waves = p.ks > 1 ? 1 : (double)((p.tiles + slots - 1) / slots);
             double t = waves * ((nkb + p.ks - 1) / p.ks) * per_kb;
-            t = (t > memory ? t : memory) + 10.0 * p.bt + (p.ks > 1 ? 2500 + 12.0 * p.bt / p.ks : 0);
+            t = (t > memory ? t : memory) + 10.0 * p.bt + (p.pair ? 4500 : 0) +
+                (p.ks > 1 ? 1500 + 400 * p.ks + 34.0 * p.bt : 0);
             if (least == 0 || t < least) {
                 least = t;
                 best = p;
