@@ -14,6 +14,7 @@
 // four more warps: TMA's tile::gather4 (four rows a copy) took 55 to 75 cycles a copy, which made a
 // batch of 4096 tokens x 6 experts (K 2688, N 3712, 64 experts) 1.12 ms against 0.34 ms.
 // Every wait is bounded; no copy names more than one CTA.
+#include <atomic>
 #include <mutex>
 #include <type_traits>
 
@@ -664,45 +665,43 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
     if (PAIR || ks > 1) cluster_sync_all();  // nobody leaves while its sums are read
 }
 
-// Clusters of `cluster` CTAs of a kernel (shared memory set) that the current device runs at once; asked
-// of the runtime once a device.
-static int clusters_at_once(const void *kern, int threads, size_t smem, int pair, int ks, int *cache) {
-    if (*cache > 0) return *cache;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(pair ? 2 : 1, 1, ks);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
+// Clusters of a dense kernel with K split ks that the current device runs at once.
+template <int BT, bool PAIR>
+static int clusters_at_once(int ks) {
+    const void *kern = (const void *)s8_gemm_kernel<BT, kDense, PAIR>;
+    const size_t smem = Cfg<BT, PAIR>::smem(0);
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = pair ? 2 : 1;
+    at[0].val.clusterDim.x = PAIR ? 2 : 1;
     at[0].val.clusterDim.y = 1;
     at[0].val.clusterDim.z = ks;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(PAIR ? 2 : 1, 1, ks);
+    cfg.blockDim = dim3(threads_of(BT, kDense));
+    cfg.dynamicSmemBytes = smem;
     cfg.attrs = at;
     cfg.numAttrs = 1;
     int n = 0;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
         cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
         (void)cudaGetLastError();
-        n = num_sms() / (ks * (pair ? 2 : 1)) / 2;  // a careful guess
+        n = num_sms() / (ks * (PAIR ? 2 : 1)) / 2;  // a careful guess
     }
-    *cache = n > 0 ? n : 1;
-    return *cache;
+    return n > 0 ? n : 1;
 }
-// Of the dense kernels, by plan: tile c (16, 64, 128, 256, pair) and K split.
-static int dense_clusters(int c, int ks) {
-    static std::mutex mu;
-    static int cache[16][5][9] = {};
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 16) dev = 0;
-    std::lock_guard<std::mutex> lk(mu);
-    int *at = &cache[dev][c][ks];
-    switch (c) {
-        case 0: return clusters_at_once((const void *)s8_gemm_kernel<16, kDense, false>, threads_of(16, kDense), Cfg<16, false>::smem(0), 0, ks, at);
-        case 1: return clusters_at_once((const void *)s8_gemm_kernel<64, kDense, false>, threads_of(64, kDense), Cfg<64, false>::smem(0), 0, ks, at);
-        case 2: return clusters_at_once((const void *)s8_gemm_kernel<128, kDense, false>, threads_of(128, kDense), Cfg<128, false>::smem(0), 0, ks, at);
-        case 3: return clusters_at_once((const void *)s8_gemm_kernel<256, kDense, false>, threads_of(256, kDense), Cfg<256, false>::smem(0), 0, ks, at);
-        default: return clusters_at_once((const void *)s8_gemm_kernel<256, kDense, true>, threads_of(256, kDense), Cfg<256, true>::smem(0), 1, ks, at);
-    }
+// The same by plan: tile c (16, 64, 128, 256, pair); asked of the runtime once a device.
+static int dense_clusters(int dev, int c, int ks) {
+    static std::atomic<int> cache[16][5][9];
+    std::atomic<int> *at = dev < 16 ? &cache[dev][c][ks] : nullptr;
+    int n = at ? at->load(std::memory_order_relaxed) : 0;
+    if (n > 0) return n;
+    n = c == 0   ? clusters_at_once<16, false>(ks)
+        : c == 1 ? clusters_at_once<64, false>(ks)
+        : c == 2 ? clusters_at_once<128, false>(ks)
+        : c == 3 ? clusters_at_once<256, false>(ks)
+                 : clusters_at_once<256, true>(ks);
+    if (at) at->store(n, std::memory_order_relaxed);
+    return n;
 }
 
 template <int BT, int MODE, bool PAIR = false>
@@ -752,8 +751,8 @@ struct Plan {
 // CTAs, four k-blocks each at least, one tile a cluster, all clusters at once) costs its exchange; and
 // nothing is faster than memory.  Within 2 % of the best of all plans on most of the shapes, 15 % off at worst
 // (150 x 4096 x 1024).
-static Plan plan_for(int M, int N, int K) {
-    const int nsm = num_sms(), nkb = (K + BK - 1) / BK;
+static Plan plan_for(int M, int N, int K, int dev, int nsm) {
+    const int nkb = (K + BK - 1) / BK;
     Plan best = {};
     double least = 0;
     const double memory = ((double)N * K + (double)M * K + 2.0 * M * N) / 3500;  // cycles at 6.5 TB/s
@@ -770,7 +769,7 @@ static Plan plan_for(int M, int N, int K) {
         double per_kb = p.pair ? (256 + p.bt > 2 * p.bt ? 256 + p.bt : 2 * p.bt) : 1.1 * (256 + 2 * p.bt);
         per_kb = per_kb > 500 ? per_kb : 500;
         for (p.ks = 1; p.ks <= (p.pair ? 4 : 8); ++p.ks) {
-            if (p.ks > 1 && (p.tiles * p.ks > slots || nkb / p.ks < 4 || p.tiles > dense_clusters(c, p.ks))) break;
+            if (p.ks > 1 && (p.tiles * p.ks > slots || nkb / p.ks < 4 || p.tiles > dense_clusters(dev, c, p.ks))) break;
             const double waves = p.ks > 1 ? 1 : (double)((p.tiles + slots - 1) / slots);
             double t = waves * ((nkb + p.ks - 1) / p.ks) * per_kb;
             t = (t > memory ? t : memory) + 10.0 * p.bt + (p.pair ? 4500 : 0) +
@@ -794,7 +793,10 @@ static int map_failed() {
 int s8_gemm(const int8_t *a, const float *a_scale, const int8_t *w, const float *w_scale, const float *bias, void *c,
             int c_dtype, int M, int N, int K, cudaStream_t st) {
     using namespace s8g;
-    const Plan p = plan_for(M, N, K);
+    int dev = 0;
+    W4_CUDA_TRY(cudaGetDevice(&dev));
+    const int nsm = num_sms();
+    const Plan p = plan_for(M, N, K, dev, nsm);
     const Args g = {a, a_scale, w_scale, bias, nullptr, nullptr, c, c_dtype, M, M, N, K, 1, p.bt,
                     p.pair ? p.bt / 2 : p.bt, p.ntn, N % 2 == 0 && aligned(c, 4), N % 4 == 0 && aligned(c, 8)};
     CUtensorMap w_map, a_map;
@@ -803,7 +805,7 @@ int s8_gemm(const int8_t *a, const float *a_scale, const int8_t *w, const float 
         !make_map_2d(&a_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, a, K, M, K, BK, g.box, CU_TENSOR_MAP_SWIZZLE_128B))
         return map_failed();
     W4_REQUIRE(p.tiles < (1L << 30), W4_ERR_UNSUPPORTED, "s8 GEMM: %ld tiles", p.tiles);
-    const int slots = p.pair ? num_sms() / 2 : num_sms();
+    const int slots = p.pair ? nsm / 2 : nsm;
     return launch_bt<kDense>(p.BT, p.pair, w_map, a_map, g, (int)(p.tiles < slots ? p.tiles : slots), p.ks, st);
 }
 
@@ -824,7 +826,7 @@ int s8_gemm_grouped(const int8_t *a, int a_rows, const float *a_scale, const int
         return map_failed();
     const long most = ((long)R / g.bt + (R < E ? R : E)) * g.ntn;  // tiles at most, whatever the counts
     W4_REQUIRE(most < (1L << 30), W4_ERR_UNSUPPORTED, "s8 GEMM: %ld tiles", most);
-    const int slots = pair ? num_sms() / 2 : num_sms(), grid = (int)(most < slots ? most : slots);
+    const int nsm = num_sms(), slots = pair ? nsm / 2 : nsm, grid = (int)(most < slots ? most : slots);
     return src ? launch_bt<kGathered>(BT, pair, w_map, a_map, g, grid, 1, st)
                : launch_bt<kGrouped>(BT, pair, w_map, a_map, g, grid, 1, st);
 }
