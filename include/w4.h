@@ -348,6 +348,8 @@ int w4_rowscale_fp8(const void *y, int y_dtype, uint8_t *q, float *row_scale, in
 /* 8-bit integer (W8A8) linears and the MoE layer around them             */
 /* ===================================================================== */
 
+/* Sizes below: at most 2^30 tokens (rows) a call, besides what each function states. */
+
 /* Function applied to the input of w4_quant_s8 before it is quantised. */
 enum w4_quant_fn {
     W4_FN_NONE = 0,     /* y = x                                                   x [M, K]  */
@@ -438,7 +440,7 @@ int w4_moe_route(const void *logits, int logits_dtype, const float *bias, int T,
  *   out[t] = add[t] + sum_j weights[t, j] * y[slots[t, j]]
  * y [rows, H] of y_dtype, out and add (or NULL) [T, H] of out_dtype, each f16 / bf16 / f32.  A slot
  * outside [0, rows) counts as a row of zeros.  out may be add; it must not overlap y.
- * 1 <= top_k <= 32, T >= 0, any H. */
+ * 1 <= top_k <= 32, T >= 0, 1 <= H <= 2^22. */
 int w4_moe_combine(const void *y, int y_dtype, int rows, const int32_t *slots, const float *weights,
                    const void *add, void *out, int out_dtype, int T, int top_k, int H, void *stream);
 

@@ -30,7 +30,7 @@ def test_quant_s8_refusals():
     assert rc(_3=_f(0x10008)) == L.W4_ERR_INVALID
     assert rc(_5=-1) == L.W4_ERR_INVALID
     assert rc(_6=0) == L.W4_ERR_INVALID
-    assert rc(_6=24) == L.W4_ERR_UNSUPPORTED
+    assert rc(_6=24) == L.W4_ERR_UNSUPPORTED and rc(_5=2**30 + 1) == L.W4_ERR_UNSUPPORTED
     assert rc(_0=None, _3=None, _4=None, _5=0) == L.W4_OK  # no rows: nothing to do
 
 
@@ -76,6 +76,7 @@ def test_moe_route_refusals():
     assert rc(_4=32, _7=32, _8=8, _9=1) == L.W4_ERR_INVALID  # top 2 of groups of one
     assert rc(_7=64, _8=64) == L.W4_ERR_UNSUPPORTED
     assert rc(_3=2**30) == L.W4_ERR_UNSUPPORTED          # T * top_k past 2^31
+    assert rc(_3=2**31 - 1, _5=1) == L.W4_ERR_UNSUPPORTED
     assert rc(_17=None) == L.W4_ERR_INVALID and b"workspace" in lib.w4_last_error()
     assert rc(_18=16) == L.W4_ERR_INVALID
     assert rc(_0=_f(0x10001)) == L.W4_ERR_INVALID
@@ -92,6 +93,7 @@ def test_moe_combine_refusals():
     assert rc(_1=L.W4_S8) == L.W4_ERR_INVALID and rc(_7=L.W4_E4M3) == L.W4_ERR_INVALID
     assert rc(_2=-1) == L.W4_ERR_INVALID and rc(_8=-1) == L.W4_ERR_INVALID and rc(_10=0) == L.W4_ERR_INVALID
     assert rc(_9=0) == L.W4_ERR_INVALID and rc(_9=33) == L.W4_ERR_UNSUPPORTED
+    assert rc(_10=2**22 + 1) == L.W4_ERR_UNSUPPORTED
     assert rc(_6=_f()) == L.W4_ERR_INVALID               # out is y
     assert rc(_8=0) == L.W4_OK
 
@@ -121,6 +123,7 @@ def test_s8_gemm_refusals():
         assert rc(**{f"_{i}": _f(0x10008)}) == L.W4_ERR_INVALID and b"aligned" in lib.w4_last_error()
     assert rc(_6=L.W4_S8) == L.W4_ERR_INVALID
     assert rc(_8=-1) == L.W4_ERR_INVALID and rc(_9=0) == L.W4_ERR_INVALID and rc(_10=0) == L.W4_ERR_INVALID
+    assert rc(_8=2**31 - 1) == L.W4_ERR_UNSUPPORTED and rc(_9=2**31 - 1) == L.W4_ERR_UNSUPPORTED
     assert rc(_10=72) == L.W4_ERR_UNSUPPORTED and rc(_10=131072) == L.W4_ERR_UNSUPPORTED
     assert rc(_6=L.W4_E4M3) == L.W4_ERR_INVALID and b"row_scale" in lib.w4_last_error()
     assert rc(_6=L.W4_E4M3, _7=_f()) == L.W4_ERR_INVALID and b"workspace" in lib.w4_last_error()

@@ -790,7 +790,6 @@ static int launch_combine(const void *y, int rows, const int *slots, const float
     constexpr int N = 16 / (int)sizeof(TY);
     const bool wide = H % N == 0 && aligned(y, 16) && aligned(out, 16) && aligned(add, 16);
     const int per = kCombineThreads * (wide ? N : 1), gy = (H + per - 1) / per;
-    W4_REQUIRE(gy <= 65535, W4_ERR_UNSUPPORTED, "H=%d is too long", H);
     W4_CUDA_TRY(launch_decode(wide ? combine_kernel<TY, TO, N> : combine_kernel<TY, TO, 1>, dim3(T, gy),
                               dim3(kCombineThreads), 0, st, 1, static_cast<const TY *>(y), rows, slots, weights,
                               static_cast<const TO *>(add), static_cast<TO *>(out), k, H));

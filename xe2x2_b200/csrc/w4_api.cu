@@ -622,6 +622,7 @@ int w4_rowscale_fp8(const void *y, int y_dtype, uint8_t *q, float *row_scale, in
 
 // ------------------------------------------------------------------ 8-bit integer linears, MoE
 static bool float_dtype(int dt) { return dt == W4_F16 || dt == W4_BF16 || dt == W4_F32; }
+constexpr int kMaxRows = 1 << 30;  // tokens of a call: counts of tiles and blocks stay in 32 bits
 
 int w4_quant_s8(const void *x, int x_dtype, int fn, int8_t *q, float *scale, int M, int K, void *stream) {
     w4::set_error("");
@@ -630,6 +631,7 @@ int w4_quant_s8(const void *x, int x_dtype, int fn, int8_t *q, float *scale, int
                "fn %d is not one of W4_FN_*", fn);
     W4_REQUIRE(M >= 0 && K > 0, W4_ERR_INVALID, "M=%d K=%d", M, K);
     W4_REQUIRE(K % 16 == 0 && K <= (1 << 28), W4_ERR_UNSUPPORTED, "K=%d must be a multiple of 16, at most 2^28", K);
+    W4_REQUIRE(M <= kMaxRows, W4_ERR_UNSUPPORTED, "M=%d exceeds 2^30", M);
     if (M == 0) return W4_OK;
     W4_REQUIRE(x && q && scale, W4_ERR_INVALID, "null pointer argument");
     W4_REQUIRE(aligned(x, 16) && aligned(q, 16) && aligned(scale, 4), W4_ERR_INVALID,
@@ -661,6 +663,7 @@ static int check_s8_shape(int c_dtype, int rows, int N, int K) {
     W4_REQUIRE(float_dtype(c_dtype) || c_dtype == W4_E4M3, W4_ERR_INVALID, "c_dtype must be f16, bf16, f32 or e4m3");
     W4_REQUIRE(rows >= 0 && N >= 1 && K >= 1, W4_ERR_INVALID, "rows=%d N=%d K=%d", rows, N, K);
     W4_REQUIRE(K % 16 == 0 && K <= 131056, W4_ERR_UNSUPPORTED, "K=%d must be a multiple of 16, at most 131056", K);
+    W4_REQUIRE(rows <= kMaxRows && N <= kMaxRows, W4_ERR_UNSUPPORTED, "rows=%d and N=%d must be at most 2^30", rows, N);
     return W4_OK;
 }
 
@@ -706,7 +709,7 @@ int w4_s8_gemm_grouped(const int8_t *a, const float *a_scale, int a_rows, const 
 }
 
 size_t w4_moe_route_workspace_bytes(int T, int E) {
-    if (T <= 0 || E < 1 || E > w4::kMaxMoeExperts) return 0;
+    if (T <= 0 || T > kMaxRows || E < 1 || E > w4::kMaxMoeExperts) return 0;
     return w4::moe_route_workspace(T, E);
 }
 
@@ -731,7 +734,8 @@ int w4_moe_route(const void *logits, int logits_dtype, const float *bias, int T,
                "W4_GROUP_TOP2 needs at least two experts a group");
     W4_REQUIRE(top_k <= topk_group * (E / groups), W4_ERR_INVALID, "top_k=%d experts out of %d that can be chosen",
                top_k, topk_group * (E / groups));
-    W4_REQUIRE((long long)T * top_k <= 0x7FFFFFFFLL, W4_ERR_UNSUPPORTED, "T * top_k exceeds 2^31 - 1");
+    W4_REQUIRE(T <= kMaxRows && (long long)T * top_k <= 0x7FFFFFFFLL, W4_ERR_UNSUPPORTED,
+               "T=%d exceeds 2^30 or T * top_k 2^31 - 1", T);
     const bool plan = offsets || rows || slots;
     if (T == 0 && !offsets) return W4_OK;
     W4_REQUIRE(T == 0 || (logits && ids && weights), W4_ERR_INVALID, "logits, ids and weights are required");
@@ -756,6 +760,7 @@ int w4_moe_combine(const void *y, int y_dtype, int rows, const int32_t *slots, c
     W4_REQUIRE(T >= 0 && rows >= 0 && H >= 1 && top_k >= 1, W4_ERR_INVALID, "T=%d rows=%d H=%d top_k=%d", T, rows, H,
                top_k);
     W4_REQUIRE(top_k <= w4::kMaxTopK, W4_ERR_UNSUPPORTED, "top_k=%d exceeds %d", top_k, w4::kMaxTopK);
+    W4_REQUIRE(H <= (1 << 22), W4_ERR_UNSUPPORTED, "H=%d exceeds 2^22", H);
     if (T == 0) return W4_OK;
     W4_REQUIRE((y || rows == 0) && slots && weights && out, W4_ERR_INVALID, "null pointer argument");
     W4_REQUIRE(out != y, W4_ERR_INVALID, "out must not be y");

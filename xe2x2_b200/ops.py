@@ -16,6 +16,9 @@ weight-only quantized linear path (hotschmoe/xe2x2):
   (kernels/epilogue_quant/rmsnorm_epilogue.cpp:118-119).
 * ``gptq_gemm(...)`` -- the W4A16 GPTQ GEMM on checkpoint tensors
   (qweight / qzeros / scales / g_idx as read by kernels/nvfp4/gptq_s4_dump.py:106).
+* ``quant_s8``, ``s8_gemm``, ``s8_gemm_grouped``, ``moe_route``, ``moe_combine`` -- 8-bit integer
+  (W8A8) linears and the mixture-of-experts layer around them; ``S8Linear`` and ``S8Experts``
+  run them together.
 
 Every function launches on the current CUDA stream and raises ``W4Error`` on
 a bad argument; there is no CPU path.

@@ -73,10 +73,16 @@ def nvfp4_bytes(M, K, N):
     return N * K // 2 + K // 16 * N + 4 + M * K * 2 + M * N * 2
 
 
+def s8_bytes(M, K, N):
+    return N * K + 4 * N + M * K + 4 * M + M * N * 2
+
+
 def main(argv=None):
     ap = argparse.ArgumentParser()
-    ap.add_argument("--kernel", choices=["gptq", "nvfp4", "producer", "gptq_grouped", "nvfp4_grouped"],
+    ap.add_argument("--kernel", choices=["gptq", "nvfp4", "producer", "s8", "gptq_grouped", "nvfp4_grouped",
+                                             "s8_grouped"],
                     default="gptq", help="producer: the fused RMSNorm -> NVFP4 activation kernel on [M, K]; "
+                    "s8: the W8A8 GEMM on quantised activations; "
                     "*_grouped: one grouped (MoE) launch over len(--counts) experts")
     ap.add_argument("--counts", default="1,1,0,1,1,1,0,1", help="tokens per expert of a grouped launch")
     ap.add_argument("--M", default="16", help="comma-separated token counts")
@@ -92,7 +98,7 @@ def main(argv=None):
     dev = torch.device("cuda:0")
     dt = torch.bfloat16 if args.dtype == "bf16" else torch.float16
     K, N = args.K, args.N
-    wbytes = gptq_bytes(0, K, N, args.gs) if args.kernel == "gptq" else nvfp4_bytes(0, K, N)
+    wbytes = {"gptq": gptq_bytes(0, K, N, args.gs), "s8": s8_bytes(0, K, N)}.get(args.kernel, nvfp4_bytes(0, K, N))
     if args.kernel.endswith("_grouped"):
         return grouped(args, dev, dt)
     if args.kernel == "producer":
@@ -104,12 +110,15 @@ def main(argv=None):
     elif args.kernel == "producer":
         copies = 1  # no weights; inputs are the activations
         ws = [None]
+    elif args.kernel == "s8":
+        ws = [synth.s8_weights(N, K, seed=s, device=dev) for s in range(copies)]
     else:
         ws = [synth.nvfp4_weights(K, N, seed=s, device=dev) for s in range(copies)]
     results = []
     for M in [int(m) for m in args.M.split(",")]:
         a = synth.activations(M, K, dt, seed=M, device=dev)
         ag = torch.tensor([float(a.float().abs().max()) / (448.0 * 6.0)], dtype=torch.float32, device=dev)
+        aq, asc = ops.quant_s8(a) if args.kernel == "s8" else (None, None)
         act_mode = L.W4_ACT_NVFP4 if args.act == "nvfp4" else L.W4_ACT_W4A16
 
         def run(i):
@@ -118,6 +127,8 @@ def main(argv=None):
                 return ops.gptq_gemm(a, w[0], w[1], w[2], args.gs, 1)
             if args.kernel == "producer":
                 return ops.rmsnorm_quant_nvfp4(a, ag)
+            if args.kernel == "s8":
+                return ops.s8_gemm(aq, asc, w[0], w[1], out_dtype=dt)
             return ops.nvfp4_gemm(a, w[0], w[1], w[2], act_mode=act_mode, a_global=ag)
 
         if not args.time:
@@ -129,7 +140,7 @@ def main(argv=None):
             run(i)
         us = statistics.median(time_launches(run, max(args.iters, 20)))
         gus = time_graph(run, max(args.iters, 20, copies))
-        nb = gptq_bytes(M, K, N, args.gs) if args.kernel == "gptq" else nvfp4_bytes(M, K, N)
+        nb = {"gptq": gptq_bytes(M, K, N, args.gs), "s8": s8_bytes(M, K, N)}.get(args.kernel, nvfp4_bytes(M, K, N))
         if args.kernel == "producer":
             nb = 2 * M * K + M * K // 2 + M * K // 16
         results.append({"kernel": args.kernel, "M": M, "K": K, "N": N, "us": round(us, 3), "graph_us": round(gus, 3),
@@ -147,7 +158,7 @@ def grouped(args, dev, dt):
     off = [0]
     for c in cnt:
         off.append(off[-1] + c)
-    a = synth.activations(off[-1], K, dt if args.kernel == "gptq_grouped" else torch.bfloat16, seed=1, device=dev)
+    a = synth.activations(off[-1], K, torch.bfloat16 if args.kernel == "nvfp4_grouped" else dt, seed=1, device=dev)
     if args.kernel == "gptq_grouped":
         ws = [synth.gptq_weights(K, N, args.gs, asym=True, seed=e, device=dev)[:3] for e in range(E)]
         qw, qz, sc = (torch.stack([w[i] for w in ws]).contiguous() for i in range(3))
@@ -155,6 +166,14 @@ def grouped(args, dev, dt):
         def run(i):
             return ops.gptq_gemm_grouped(a, qw, qz, sc, off, args.gs, 1)
         nb = sum(1 for c in cnt if c) * gptq_bytes(0, K, N, args.gs)
+    elif args.kernel == "s8_grouped":
+        w, sc = (torch.stack(t).contiguous() for t in zip(*(synth.s8_weights(N, K, seed=e, device=dev) for e in range(E))))
+        q, s = ops.quant_s8(a)
+        offsets = torch.tensor(off, dtype=torch.int32, device=dev)
+
+        def run(i):
+            return ops.s8_gemm_grouped(q, s, w, sc, offsets, out_dtype=dt)
+        nb = sum(1 for c in cnt if c) * s8_bytes(0, K, N)
     else:
         ws = [synth.nvfp4_weights(K, N, seed=e, device=dev) for e in range(E)]
         w_nk = torch.stack([w[0].t() for w in ws]).contiguous()

@@ -6,6 +6,7 @@ layout), zeros uniform 0..15 packed along N (or none = symmetric),
 scales fp16 = |N(0, 0.02)| + 1e-3 per (group, column), activations ~N(0, sigma).
 NVFP4: codes uniform over the 16 E2M1 values, two per byte; E4M3 block scales
 = e4m3(2^u), u ~ U[-6, 2]; fp32 tensor scale 1/448; activations bf16 ~N(0, 1).
+S8: weights N(0, 1) / sqrt(K) quantised to int8 with an f32 scale per output channel.
 Uniform random 32-bit words have uniform independent nibbles, so packed
 tensors are drawn directly as random words / bytes.
 """
@@ -51,6 +52,13 @@ def nvfp4_weights(K: int, N: int, seed: int = 0, device="cpu"):
     scale = torch.exp2(u).to(torch.float8_e4m3fn)
     gscale = torch.full((1,), 1.0 / 448.0, dtype=torch.float32, device=device)
     return w_nk.t(), scale, gscale
+
+
+def s8_weights(N: int, K: int, seed: int = 0, device="cpu"):
+    """-> (w s8 [N, K], per-channel scale f32 [N]): N(0, 1) / sqrt(K) rounded to 127 steps of its maximum."""
+    w = torch.randn((N, K), generator=_gen(seed, device), device=device) / K ** 0.5
+    scale = w.abs().amax(1) / 127.0
+    return torch.round(w / scale[:, None]).to(torch.int8), scale
 
 
 def gptq_s4_tile(rows: int, k: int, cols: int, seed: int = 0, device="cpu"):
