@@ -105,6 +105,20 @@ def test_tiny_and_huge_rows_equal_f32_arithmetic(cuda, size):
     assert np.array_equal(np_(q).astype(np.float32), ref)
 
 
+def test_scales_of_a_few_units_clamp_the_codes(cuda):
+    """A scale of k units in the last place of the subnormals is off by up to half a unit, so max / scale
+    passes 127 (190 at k = 1): such codes are 127."""
+    k = np.arange(1, 160)[:, None]
+    units = np.concatenate([127 * k + 63, -(127 * k + 60), 64 * k, 127 * k, np.repeat(k, 12, 1)], 1).astype(np.uint32)
+    sign = np.zeros_like(units)
+    units[:, 1], sign[:, 1] = 127 * k[:, 0] + 60, 1
+    xf = np.ascontiguousarray(units | sign << np.uint32(31)).view(np.float32)
+    q, s = ops.quant_s8(torch.from_numpy(xf).to(cuda))
+    want = (np.abs(xf).max(1) / np.float32(127)).astype(np.float32)
+    assert np.array_equal(np_(s), want)
+    assert np.array_equal(np_(q), np.clip(np.rint((xf / want[:, None]).astype(np.float32)), -127, 127).astype(np.int8))
+
+
 def test_halves_of_the_maximum_round_to_even(cuda):
     """x = max / 2 is a tie in real arithmetic (63.5): decided as y / s rounds in f32."""
     for dt in DTYPES.values():

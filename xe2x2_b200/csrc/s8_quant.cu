@@ -128,10 +128,12 @@ __device__ __forceinline__ Scale scale_of(uint32_t top) {
 __device__ __forceinline__ uint2 quant8(const float (&y)[8], const Scale &c) {
     if (!c.finite) return make_uint2(0u, 0u);
     if (c.s >= 1e-30f) return codes8(y, c.s, c.inv);
-    float z[8];  // a scale whose reciprocal may overflow: the same quotients, both sides times 2^100
+    // A scale whose reciprocal may overflow: the same quotients, both sides times 2^100.  A subnormal scale
+    // may have rounded down by more than the last code's half: the quotient is held to 127.
+    const float s = c.s * 0x1p100f, most = 127.f * s;
+    float z[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) z[i] = y[i] * 0x1p100f;
-    const float s = c.s * 0x1p100f;
+    for (int i = 0; i < 8; ++i) z[i] = fminf(fmaxf(y[i] * 0x1p100f, -most), most);
     return codes8(z, s, __fdiv_rn(1.f, s));
 }
 
