@@ -157,3 +157,24 @@ def test_s8_wrapper_refusals():
         ops.s8_gemm(a, s, w[0], ws)
     with pytest.raises(ValueError):
         ops.s8_gemm_grouped(a, s, w, ws, torch.zeros(2, dtype=torch.int32))
+
+
+def test_sizes_past_32_bits_are_refused_before_the_call():
+    """A size of 2^32 + 64 would arrive as 64."""
+    big = 2**32 + 64
+
+    def meta(*shape, dtype=torch.int8):
+        return torch.empty(shape, dtype=dtype, device="meta")
+
+    s1 = meta(1, dtype=torch.float32)
+    off = torch.zeros(2, dtype=torch.int32)
+    for call in (lambda: ops.quant_s8(meta(1, big, dtype=torch.float16)),
+                 lambda: ops.quant_s8(meta(big, 16, dtype=torch.float16)),
+                 lambda: ops.s8_gemm(meta(big, 16), s1, meta(1, 16), s1),
+                 lambda: ops.s8_gemm(meta(1, 16), s1, meta(big, 16), s1),
+                 lambda: ops.s8_gemm_grouped(meta(big, 16), s1, meta(1, 1, 16), s1, off),
+                 lambda: ops.moe_route(meta(big, 1, dtype=torch.float16), 1),
+                 lambda: ops.moe_route(meta(1, 64, dtype=torch.float16), 1, n_group=2**32 + 1),
+                 lambda: ops.moe_combine(meta(1, big), meta(1, 1), meta(1, 1))):
+        with pytest.raises(ValueError, match="2\\^31"):
+            call()

@@ -413,6 +413,12 @@ def _arg(t, name, dtypes, shape, dev, optional=False):
     raise ValueError(f"{name} must be contiguous")
 
 
+def _sizes(*n):
+    """Refuse sizes that the entry points' 32-bit arguments would cut off."""
+    if max(n) > 0x7FFFFFFF:
+        raise ValueError(f"sizes must be below 2^31, got {max(n)}")
+
+
 def _call_on(dev, name, *args):
     """Call an entry point on the current stream of device index dev, with dev as the current device."""
     if dev == torch.cuda.current_device():
@@ -436,6 +442,7 @@ def quant_s8(x, act=None):
         raise ValueError("x must be a 2-D tensor")
     dev, fn = x.get_device(), _FN[act]
     M, K = x.shape
+    _sizes(M, K)
     px = _arg(x, "x", _FLOATS, (M, K), dev)
     if fn == L.W4_FN_SILU_MUL:
         if K % 2:
@@ -483,6 +490,7 @@ def s8_gemm(a, a_scale, w, w_scale, bias=None, out_dtype=None, out=None):
         raise ValueError("a must be [M, K] and w [N, K]")
     dev = a.get_device()
     (M, K), N = a.shape, w.shape[0]
+    _sizes(M, N, K)
     pa, pas = _arg(a, "a", _S8, (M, K), dev), _arg(a_scale, "a_scale", _F32, (M,), dev)
     pw, pws = _arg(w, "w", _S8, (N, K), dev), _arg(w_scale, "w_scale", _F32, (N,), dev)
     pb = _arg(bias, "bias", _F32, (N,), dev, optional=True)
@@ -505,6 +513,7 @@ def s8_gemm_grouped(a, a_scale, w, w_scale, offsets, rows=None, bias=None, out_d
         raise ValueError("a must be [tokens, K] and w [E, N, K]")
     dev = a.get_device()
     (A, K), (E, N, _) = a.shape, w.shape
+    _sizes(A, E, N, K)
     pa, pas = _arg(a, "a", _S8, (A, K), dev), _arg(a_scale, "a_scale", _F32, (A,), dev)
     pw, pws = _arg(w, "w", _S8, (E, N, K), dev), _arg(w_scale, "w_scale", _F32, (E, N), dev)
     pb = _arg(bias, "bias", _F32, (E, N), dev, optional=True)
@@ -513,6 +522,7 @@ def s8_gemm_grouped(a, a_scale, w, w_scale, offsets, rows=None, bias=None, out_d
         if not torch.is_tensor(rows) or rows.dim() != 1:
             raise ValueError("rows must be a 1-D tensor")
         R = rows.shape[0]
+        _sizes(R)
         pr = _arg(rows, "rows", _I32, (R,), dev)
     c, cdt, rs, ws = _s8_out(a, R, N, out_dtype, out, dev)
     _call_on(dev, "w4_s8_gemm_grouped", pa, pas, A, pw, pws, pb, po, pr, E, c.data_ptr(), cdt, _ptr(rs), R, N, K,
@@ -570,9 +580,10 @@ def moe_route(logits, top_k, bias=None, score="softmax", renormalize=True, scali
         raise ValueError("logits must be a 2-D tensor [tokens, experts]")
     dev = logits.get_device()
     T, E = logits.shape
+    top_k, n_group, topk_group = int(top_k), int(n_group), int(topk_group)
+    _sizes(T, E, top_k, n_group, topk_group)
     pl = _arg(logits, "logits", _FLOATS, (T, E), dev)
     pb = _arg(bias, "bias", _F32, (E,), dev, optional=True)
-    top_k = int(top_k)
     if top_k < 1:
         raise ValueError(f"top_k must be at least 1, got {top_k}")
     i32 = torch.int32
@@ -581,8 +592,8 @@ def moe_route(logits, top_k, bias=None, score="softmax", renormalize=True, scali
     offsets, rows = logits.new_empty(E + 1, dtype=i32), logits.new_empty(T * top_k, dtype=i32)
     need = L.lib().w4_moe_route_workspace_bytes(T, E)
     ws = logits.new_empty(need, dtype=torch.uint8) if need else None
-    _call_on(dev, "w4_moe_route", pl, _FLOATS[logits.dtype], pb, T, E, top_k, _SCORES[score], int(n_group),
-             int(topk_group), _GROUP_SCORES[group_score], int(bool(renormalize)), float(scaling), ids.data_ptr(),
+    _call_on(dev, "w4_moe_route", pl, _FLOATS[logits.dtype], pb, T, E, top_k, _SCORES[score], n_group,
+             topk_group, _GROUP_SCORES[group_score], int(bool(renormalize)), float(scaling), ids.data_ptr(),
              weights.data_ptr(), offsets.data_ptr(), rows.data_ptr(), slots.data_ptr(), _ptr(ws), need)
     return MoERouting(ids, weights, offsets, rows, slots)
 
@@ -596,6 +607,7 @@ def moe_combine(y, slots, weights, add=None, out_dtype=None):
         raise ValueError("y must be [rows, H] and slots [tokens, top_k]")
     dev = y.get_device()
     (rows, H), (T, k) = y.shape, slots.shape
+    _sizes(rows, H, T, k)
     out_dtype = out_dtype or y.dtype
     py, ps = _arg(y, "y", _FLOATS, (rows, H), dev), _arg(slots, "slots", _I32, (T, k), dev)
     pw = _arg(weights, "weights", _F32, (T, k), dev)
