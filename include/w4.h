@@ -363,7 +363,8 @@ enum w4_quant_fn {
  * in f32 and never rounded to x_dtype.  A row in which y has a NaN or an infinity gets that
  * as its scale and zero codes, so products with it are NaN.  The arithmetic is that of
  * w4_rmsnorm_quant_s8 without the norm (kernels/epilogue_quant/rmsnorm_epilogue.cpp:56-70); with
- * W4_FN_SILU_MUL y is within about 1e-6 (relative) of the formula.
+ * W4_FN_SILU_MUL y is within about 1e-6 (relative) of the formula for gates down to -8, within
+ * |g| 2^-24 more below, and 0 below -87 (where 1 / (1 + exp(-g)) leaves f32's normal range).
  * K % 16 == 0, x and q 16-byte aligned and not overlapping, M >= 0. */
 int w4_quant_s8(const void *x, int x_dtype, int fn, int8_t *q, float *scale, int M, int K, void *stream);
 

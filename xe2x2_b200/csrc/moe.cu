@@ -653,9 +653,9 @@ __global__ void __launch_bounds__(KT) place_kernel(const RouteArgs a) {
 }
 
 // Threads and tokens of a CTA.  Up to 32 tokens one CTA does everything.  Up to 16 an SM: 16 warps, a token
-// each (148 tokens: 8.4 us, with 32 warps 11.6).  More: one CTA of 32 warps an SM (8192 tokens: 25 us, with
-// two of 16 warps 28, since every CTA of the second kernel reads all counts); at most 1024 tokens (the
-// masks are E * chunk / 8 bytes of shared memory).
+// each (148 tokens: 8.4 us, with 32 warps 11.6).  More: one CTA of 32 warps an SM (8192 tokens: 25 us where
+// two of 16 warps took 28, since every CTA of the second kernel reads all counts; 20 us since); at most 1024
+// tokens (the masks are E * chunk / 8 bytes of shared memory).
 struct Shape {
     int threads, chunk;
 };
