@@ -300,3 +300,28 @@ def test_every_choice_of_many_tokens_is_the_64_bit_one(cuda, E, score, G, tg, gr
     w = p.gather(1, ids)
     w = w / w.sum(1, keepdim=True)
     assert float(((r.weights.double() - w) / w).abs().max()) < 1e-5
+
+
+def test_threads_with_calls_of_different_sizes(cuda):
+    """Calls that take much and little shared memory, from threads at once, do not refuse each other."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    g = torch.Generator(device=cuda).manual_seed(8)
+    big = torch.randn(40000, 480, generator=g, device=cuda)     # 32 groups of 15: masks and scratch
+    small = torch.randn(3000, 480, generator=g, device=cuda)
+    calls = [(big, 8), (small, 8), (small, 4), (big, 2)]
+    torch.cuda.synchronize()
+
+    def run(logits, k):
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            for _ in range(50):
+                r = ops.moe_route(logits, k, score="sigmoid", n_group=32, topk_group=5, group_score="top2")
+        side.synchronize()
+        return r
+
+    want = [run(*c) for c in calls]
+    with ThreadPoolExecutor(4) as pool:
+        got = list(pool.map(lambda c: run(*c), calls))
+    for r, w in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(r, w))

@@ -678,14 +678,19 @@ static cudaError_t launch_route(const RouteArgs &a, int chunks, size_t masks, si
         case 8: kern = route_kernel<8, KT>; break;
         default: kern = route_kernel<16, 512>;
     }
-    if (smem > 16384) {  // above the default limit less the static arrays
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    // Above the default limit less the static arrays: what any call takes, so that a smaller call from
+    // another thread does not lower the limit before this one's launch.
+    constexpr int kMost = kMaxMoeExperts * 1024 / 8 + 16 + 32 * (256 + 8) * 8;
+    static_assert(16 * (kMaxMoeExperts + kMaxMoeExperts / 32) <= 32 * (256 + 8), "512 threads above 256 experts");
+    if (smem > 16384) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
         if (e != cudaSuccess) return e;
     }
     cudaError_t e = launch_decode(kern, dim3(chunks), dim3(KT), smem, st, 1, a);
     if (e != cudaSuccess || !a.counts) return e;
     if (masks > 32768)
-        e = cudaFuncSetAttribute(place_kernel<KT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)masks);
+        e = cudaFuncSetAttribute(place_kernel<KT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 kMaxMoeExperts * 1024 / 8);
     return e != cudaSuccess ? e : launch_decode(place_kernel<KT>, dim3(chunks), dim3(KT), masks, st, 1, a);
 }
 
