@@ -92,9 +92,9 @@ __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 // The same barrier in CTA `rank` of the cluster, as a shared::cluster address; an arrival there.  The
-// default scope: what an arrival passes on is written and read by the copy engine and the tensor
-// core, ordered by their own completion mechanisms and proxy fences.  With .release.cluster /
-// .acquire.cluster on these barriers M = 8192, K = 5120, N = 17408 took 977 us instead of 519.
+// default scope (the CTA): such an arrival passes on that the tensor core has finished with a stage or an
+// accumulator, or that a read of TMEM has (tcgen05.commit, tcgen05.wait), and nothing that threads wrote.
+// Rows that threads wrote go by publish_rows / observe_rows.
 __device__ __forceinline__ uint32_t bar_of(uint64_t *bar, uint32_t rank) {
     uint32_t a;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(bar)), "r"(rank));
@@ -189,15 +189,42 @@ __device__ __forceinline__ uint32_t idesc_for(int n, int m) {
     return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
+// Token rows that threads of one CTA copied into its shared memory, read by MMAs that a thread of the other
+// CTA issues: the arrival and the wait that see each other need cluster scope, and so does the order around
+// them.  The fences' .sync_restrict forms order accesses to shared memory alone, which is all there is:
+// 4096 tokens x 6 of 64 experts, K = 2688, N = 3712 take 257 us; with .release.cluster on the arrival
+// and .acquire.cluster on the wait 314, with fence.acq_rel.cluster behind the wait 573.
+__device__ __forceinline__ void publish_rows(uint32_t addr) {
+    asm volatile(
+        "fence.release.sync_restrict::shared::cta.cluster;\n\t"
+        "mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ bool try_wait_cluster(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n.reg .pred p;\nmbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, "
+        "p;\n}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+__device__ __forceinline__ void observe_rows() {
+    asm volatile("fence.acquire.sync_restrict::shared::cluster.cluster;" ::: "memory");
+}
+
 // Bounded wait.  The clock is read only after some tries: reading it costs about as much as a stage
-// of the decode GEMM takes.
+// of the decode GEMM takes.  CLUSTER: see publish_rows.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool wait_s8(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
     const uint32_t b = smem_u32(bar);
+    auto done = [&] { return CLUSTER ? try_wait_cluster(b, parity) : mbar_try_wait(b, parity); };
 #pragma unroll 1
     for (int i = 0; i < 64; ++i)
-        if (mbar_try_wait(b, parity)) return true;
+        if (done()) return true;
     const unsigned long long t0 = global_ns();
-    while (!mbar_try_wait(b, parity)) {
+    while (!done()) {
         if (*abort_flag) return false;
         if (global_ns() - t0 > kWaitLimitNs) {
             *abort_flag = 1;
@@ -291,14 +318,14 @@ __device__ __forceinline__ void store_rows(const Args &a, const uint32_t (&v)[LD
 }
 
 // A gather warp's finished stage: every lane orders its copies into its own CTA's shared memory before
-// the tensor core's reads (the .shared::cluster form of the fence: 642 us where this takes 274, batch
-// above), then one arrival (on the first CTA's barrier, where the pair's MMAs are issued).
+// the tensor core's reads (the .shared::cluster form of the fence took more than twice as long for the whole
+// kernel), then one arrival (on the first CTA's barrier, where the pair's MMAs are issued).
 template <bool PAIR>
 __device__ __forceinline__ void hand_over(uint64_t *bar, uint32_t lead, int lane) {
     fence_proxy_async();
     __syncwarp();
     if (lane == 0) {
-        if constexpr (PAIR) mbar_arrive_cluster(bar_of(bar, lead));
+        if constexpr (PAIR) publish_rows(bar_of(bar, lead));
         else mbar_arrive(bar);
     }
 }
@@ -500,6 +527,7 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
             for (int i = g > S ? g - S : 0; i < g; ++i) mbar_wait_bounded(&full[i % S], (uint32_t)((i / S) & 1));
     } else if (warp == 1 && rank == 0 && elect_one()) {
         // ---------------- MMA issuer ----------------
+        constexpr bool ROWS_BY_THREADS = PAIR && MODE == kGathered;  // those of the other CTA too
         const uint64_t d0 = sw128_desc(smem_u32(sm));
         int s = 0, j = 0;
         uint32_t phase = 0;
@@ -511,10 +539,11 @@ s8_gemm_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
             if (j >= 2 && !wait_s8(&acc_empty[j & 1], (uint32_t)((j / 2 - 1) & 1), abort_flag)) break;
             tc_fence_after();
             for (int kb = kb0; kb < kb1; ++kb) {
-                if (!wait_s8(&full[s], phase, abort_flag)) {
+                if (!wait_s8<ROWS_BY_THREADS>(&full[s], phase, abort_flag)) {
                     ok = false;
                     break;
                 }
+                if constexpr (ROWS_BY_THREADS) observe_rows();
                 tc_fence_after();
                 const uint64_t wd = d0 + (uint64_t)(s * (C_::STAGE >> 4)), td = wd + (W_BYTES >> 4);
 #pragma unroll
