@@ -1,0 +1,55 @@
+"""Choices of w4_moe_route that 32 bits cannot make alone: signed zeros, group sums that cancel, ties at
+the last rank, scores far below the largest.  Every id against the definition in 64 bits."""
+import pytest
+import torch
+
+from xe2x2_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+
+def _ids64(x, k, bias=None, score="softmax", G=1, tg=1, group_score="max"):
+    T, E = x.shape
+    xd = x.double()
+    p = torch.softmax(xd, 1) if score == "softmax" else torch.sigmoid(xd)
+    key = xd if bias is None else p + bias.double()
+    if G > 1:
+        val = p if bias is None and group_score == "top2" else key
+        best = val.view(T, G, E // G).sort(dim=2, descending=True).values
+        total = best[:, :, 0] + (best[:, :, 1] if group_score == "top2" else 0)
+        kept = total.sort(dim=1, descending=True, stable=True).indices[:, :tg]
+        on = torch.zeros(T, G, dtype=torch.bool, device=x.device).scatter_(1, kept, True)
+        key = key.masked_fill(~on.repeat_interleave(E // G, 1), -float("inf"))
+    return key.sort(dim=1, descending=True, stable=True).indices[:, :k]
+
+
+def _check(x, k, bias=None, score="softmax", G=1, tg=1, group_score="max"):
+    want = _ids64(x, k, bias, score, G, tg, group_score)
+    got = ops.moe_route(x, k, bias, score, n_group=G, topk_group=tg, group_score=group_score).ids.long()
+    wrong = (got != want).any(1)
+    assert not wrong.any(), (int(wrong.sum()), got[wrong][0].tolist(), want[wrong][0].tolist())
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+# ---------------------------------------------------------------------------- signed zeros
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_minus_zero_ties_with_zero_under_tied_groups(cuda, score):
+    x = torch.tensor([[-0.0, 0.0, -0.0, 0.0]], device=cuda)
+    assert ops.moe_route(x, 1, score=score, n_group=2, topk_group=1, group_score="top2").ids.tolist() == [[0]]
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_choices_among_mixed_zeros(cuda, dtype, score):
+    """No logit above zero, a third of them -0: the choice reaches 0 and -0."""
+    x = (torch.randint(-2, 1, (300, 64), generator=_gen(1), device=cuda) * 0.5).to(dtype)
+    x[:, ::3] = -0.0
+    zero = torch.zeros(64, device=cuda)
+    for b in (None, zero):
+        _check(x, 8, b, score)
+        for gs in ("max", "top2"):
+            _check(x, 8, b, score, 8, 3, gs)
+            _check(x, 8, b, score, 4, 1, gs)

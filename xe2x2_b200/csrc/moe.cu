@@ -303,7 +303,8 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const Token<EPL> &k, 
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < EPL; ++i) key[i] = NARROW ? k.key[i] : k.key[i] ? ordered((V)k.l[i]) : 0;
+            for (int i = 0; i < EPL; ++i)  // -0 orders as 0, as in the 32-bit keys
+                key[i] = NARROW ? k.key[i] : k.key[i] ? ordered((V)k.l[i] + (V)0) : 0;
         }
 #pragma unroll
         for (int i = 0; i < EPL; ++i) val[i] = key[i] ? s[i] : (V)-INFINITY;
