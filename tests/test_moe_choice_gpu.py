@@ -53,3 +53,17 @@ def test_choices_among_mixed_zeros(cuda, dtype, score):
         for gs in ("max", "top2"):
             _check(x, 8, b, score, 8, 3, gs)
             _check(x, 8, b, score, 4, 1, gs)
+
+
+# ---------------------------------------------------------------------------- group sums that cancel
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("size", [64.0, 4096.0])
+def test_groups_whose_two_best_cancel(cuda, size, score):
+    """Biases near +size and -size on a group's two best: the sums are of the scores' size, their 32-bit
+    errors of the biases'."""
+    T, E, G = 50_000, 64, 8
+    x = torch.randn(T, E, generator=_gen(2), device=cuda)
+    bias = torch.full((E,), -3 * size, device=cuda)
+    bias[1::8], bias[4::8] = size, -size
+    for tg in (1, 3):
+        _check(x, tg, bias, score, G, tg, "top2")

@@ -153,7 +153,10 @@ __device__ __forceinline__ bool group_kept(const RouteArgs &a, V first, V second
         const int in = __ffs(__ballot_sync(0xffffffffu, lead && rank == a.topk_group - 1)) - 1;
         const int out = __ffs(__ballot_sync(0xffffffffu, lead && rank == a.topk_group)) - 1;
         const float x = (float)__shfl_sync(0xffffffffu, total, in), y = (float)__shfl_sync(0xffffffffu, total, out);
-        *close = y > -INFINITY && x - y <= 2 * close_to(a.softmax, 1.f, x);
+        // the values' errors are of their size, not of the sum's: two large ones may cancel
+        const float size = (float)(fabs(first) + (a.top2 && second > (V)-INFINITY ? fabs(second) : (V)0));
+        const float most = fmaxf(__shfl_sync(0xffffffffu, size, in), __shfl_sync(0xffffffffu, size, out));
+        *close = y > -INFINITY && x - y <= 2 * close_to(a.softmax, 1.f, most);
     }
     return g < a.groups && rank < a.topk_group;
 }
