@@ -67,3 +67,32 @@ def test_groups_whose_two_best_cancel(cuda, size, score):
     bias[1::8], bias[4::8] = size, -size
     for tg in (1, 3):
         _check(x, tg, bias, score, G, tg, "top2")
+
+
+# ---------------------------------------------------------------------------- ties at the last rank
+def test_a_tie_at_the_last_rank_does_not_hide_a_larger_score(cuda):
+    """In 32 bits all three have the score 1; the two at 20 tie in any precision, the one at 21 is larger."""
+    x = torch.full((1, 40), -3.0, device=cuda)
+    x[0, 4] = x[0, 9] = 20.0
+    x[0, 30] = 21.0
+    zero = torch.zeros(40, device=cuda)
+    assert ops.moe_route(x, 1, zero, "sigmoid").ids.tolist() == [[30]]
+    x[0, 1] = 22.0
+    assert ops.moe_route(x, 2, zero, "sigmoid").ids.tolist() == [[1, 30]]
+
+
+@pytest.mark.parametrize("E", [48, 256, 480])
+@pytest.mark.parametrize("k", [1, 2, 6, 31, 32])
+def test_logits_on_a_grid_with_equal_scores_in_32_bits(cuda, E, k):
+    x = 18 + torch.randint(0, 24, (400, E), generator=_gen(E + k), device=cuda) * 0.5
+    zero = torch.zeros(E, device=cuda)
+    _check(x, k, zero, "sigmoid")                       # within 2^-24 of 1, up to 1 - 6e-14
+    _check(x.bfloat16(), k, zero, "sigmoid")
+    half = torch.full((E,), 0.5, device=cuda)
+    low = -38 + torch.randint(0, 30, (400, E), generator=_gen(k), device=cuda) * 0.5
+    _check(low, k, half, "sigmoid")                     # lost in the sum with the bias
+    low[:, 7] = 0.0
+    _check(low, k, half, "softmax")
+    if k <= 12:
+        _check(x, k, zero, "sigmoid", 4, 2, "top2")
+        _check(low, k, half, "softmax", 4, 2, "max")

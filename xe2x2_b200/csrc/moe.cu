@@ -383,12 +383,27 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const Token<EPL> &k, 
             const uint32_t bm = __shfl_down_sync(0xffffffffu, mine, 1);
             const int e2 = lane == a.k - 1 ? last_e : be;
             const uint32_t m2 = lane == a.k - 1 ? last : bm;
-            bool near = false;
+            bool near = false, tie = false;
             if (lane < a.k && c->e >= 0 && m2 != 0 && e2 >= 0) {
                 const float x = from_ordered(mine), y = from_ordered(m2), bx = a.bias[c->e], by = a.bias[e2];
                 // equal logits and biases are a tie in any precision
-                if (x - y <= close_to(a.softmax, fmaxf(x - bx, y - by), x))
+                if (x - y <= close_to(a.softmax, fmaxf(x - bx, y - by), x)) {
                     near = bx != by || logit_of(a, k.t, c->e) != logit_of(a, k.t, e2);
+                    tie = !near && lane == a.k - 1;
+                }
+            }
+            if (__any_sync(0xffffffffu, tie)) {
+                // The last one chosen ties with the one behind it, which says nothing of those behind that: each
+                // is compared with the last one here, and `from` for all that were not ranked.
+                const int le = __shfl_sync(0xffffffffu, c->e, a.k - 1);
+                const float x = from_ordered(__shfl_sync(0xffffffffu, mine, a.k - 1)), bx = a.bias[le];
+                near |= !done || x - from_ordered(from) <= close_to(a.softmax, 1.f, x);
+                if (done && lane > a.k && lane < n) {
+                    const uint2 o = pick->out[lane];
+                    const float y = from_ordered(o.x), by = a.bias[o.y];
+                    if (x - y <= close_to(a.softmax, fmaxf(x - bx, y - by), x))
+                        near |= bx != by || logit_of(a, k.t, le) != logit_of(a, k.t, o.y);
+                }
             }
             if (__any_sync(0xffffffffu, near)) {
                 // A sigmoid needs no other expert: if every key that could reach the top_k is among those
