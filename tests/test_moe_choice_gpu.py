@@ -96,3 +96,17 @@ def test_logits_on_a_grid_with_equal_scores_in_32_bits(cuda, E, k):
     if k <= 12:
         _check(x, k, zero, "sigmoid", 4, 2, "top2")
         _check(low, k, half, "softmax", 4, 2, "max")
+
+
+# ---------------------------------------------------------------------------- scores far below the largest
+@pytest.mark.parametrize("gap", [15.0, 30.0, 60.0, 82.0])
+def test_softmax_scores_far_below_the_largest(cuda, gap):
+    """One expert holds all of the sum; the others' scores, and biases of their size, lie as close as the
+    rounding of exp's argument (gap * 2^-24 each time it is rounded)."""
+    T, E, k = 40_000, 64, 8
+    g = _gen(int(gap))
+    x = -gap + 1.7 + 1e-3 * torch.rand(T, E, generator=g, device=cuda)
+    x[:, 11] = 1.7 + torch.rand(T, generator=g, device=cuda)
+    bias = torch.exp(torch.tensor(-gap, device=cuda)) * 5e-4 * torch.rand(E, generator=g, device=cuda)
+    _check(x, k, bias, "softmax")
+    _check(x, k, bias, "softmax", 4, 4, "max")

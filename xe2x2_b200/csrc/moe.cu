@@ -96,11 +96,13 @@ __device__ __forceinline__ float score_of(float l, bool softmax, float top, floa
 }
 // Two values further apart than this are in order although their scores were taken in 32 bits.  A sigmoid
 // of 32 bits is within 2e-7 of the exact one (2^-22 of the exponential times at most a quarter, 2^-23 of
-// the reciprocal); a softmax's terms are within 3e-6 of their size (argument and exponential, and a sum
-// of up to 512 terms).  `score` is the larger score (or sum of scores) of the two; their values round
-// once or twice more.
+// the reciprocal).  Two terms of a softmax, d = l - top below the largest, are each within 2^-22 of the
+// exponential and |d| 2^-23 of its argument, which rounds twice (log2(e) itself is common to both, but
+// for |d| 2^-26); the sum of up to 512 terms, 2.4e-6, scales both alike: 3e-6 + 2.6e-7 |d| of the larger
+// one together, and |d| is at most -log(score).  `score` is the larger score (or sum of scores) of the
+// two; their values round once or twice more.
 __device__ __forceinline__ float close_to(bool softmax, float score, float value) {
-    return (softmax ? 6e-6f * score : 1e-6f) + 5e-7f * fabsf(value);
+    return (softmax ? (4e-6f - 3e-7f * __logf(fmaxf(score, 1e-38f))) * score : 1e-6f) + 5e-7f * fabsf(value);
 }
 
 // What a warp knows of one token: its logits (-inf where an expert is off), the largest one (finite), and
