@@ -383,10 +383,10 @@ int w4_s8_gemm(const int8_t *a, const float *a_scale, const int8_t *w, const flo
 
 /* Grouped (MoE) W8A8 GEMM: expert e multiplies rows [offsets[e], offsets[e+1]) of the batch by its
  * slice of w s8 [E, N, K] with w_scale f32 [E, N] and bias f32 [E, N] or NULL; c [R, N].
- * offsets: i32 [E + 1] in DEVICE memory, nondecreasing from 0 to at most R, as w4_moe_route writes
- * them (never read by the host; values outside [0, R] or out of order are clamped, so no row
- * outside the buffers is touched).  Rows of c (and of row_scale) behind offsets[E] are left as
- * they are.
+ * offsets: i32 [E + 1] in DEVICE memory, nondecreasing, at most R, as w4_moe_route writes
+ * them (never read by the host; values outside [0, R] are clamped and one below an earlier one
+ * counts as that one, so no row outside the buffers is touched).  Rows of c (and of row_scale) before
+ * offsets[0] and behind the last expert's are left as they are.
  * rows == NULL: row r of the batch is row r of a s8 [R, K], a_rows = R.  Else row r is row rows[r] of
  * a s8 [a_rows, K] (i32 [R] in device memory, as w4_moe_route writes it), with its a_scale; an index
  * outside [0, a_rows) counts as a row of zeros.

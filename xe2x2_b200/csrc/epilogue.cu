@@ -90,10 +90,14 @@ __device__ __forceinline__ float load_as_f(const void *p, size_t i) {
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads)
 rowscale_fp8_kernel(const void *__restrict__ y, uint8_t *__restrict__ q,
-                    float *__restrict__ row_scale, int N, const int *__restrict__ limit) {
+                    float *__restrict__ row_scale, int N, const int *__restrict__ offsets, int E) {
     __shared__ float sh[32];
     const int row = blockIdx.x;
-    if (limit && row >= *limit) return;
+    if (offsets) {  // a grouped call: rows of no expert (w4_s8_gemm_grouped's order) are left alone
+        bool before_end = false;
+        for (int e = threadIdx.x; e < E; e += blockDim.x) before_end |= row < offsets[e + 1];
+        if (!__syncthreads_or(before_end) || row < offsets[0]) return;
+    }
     const size_t base = (size_t)row * N;
     float amax = 0.f;
     for (int j = threadIdx.x; j < N; j += blockDim.x) amax = fmaxf(amax, fabsf(load_as_f<T>(y, base + j)));
@@ -148,11 +152,11 @@ int rowscale_fp8_amax(const float *y, unsigned int *rowmax, unsigned int *rowcnt
 }
 
 int rowscale_fp8(const void *y, int y_dtype, uint8_t *q, float *row_scale, int M, int N,
-                 cudaStream_t st, const int *limit) {
-    if (y_dtype == W4_F32) rowscale_fp8_kernel<float><<<M, kRowThreads, 0, st>>>(y, q, row_scale, N, limit);
+                 cudaStream_t st, const int *offsets, int E) {
+    if (y_dtype == W4_F32) rowscale_fp8_kernel<float><<<M, kRowThreads, 0, st>>>(y, q, row_scale, N, offsets, E);
     else if (y_dtype == W4_BF16)
-        rowscale_fp8_kernel<__nv_bfloat16><<<M, kRowThreads, 0, st>>>(y, q, row_scale, N, limit);
-    else rowscale_fp8_kernel<__half><<<M, kRowThreads, 0, st>>>(y, q, row_scale, N, limit);
+        rowscale_fp8_kernel<__nv_bfloat16><<<M, kRowThreads, 0, st>>>(y, q, row_scale, N, offsets, E);
+    else rowscale_fp8_kernel<__half><<<M, kRowThreads, 0, st>>>(y, q, row_scale, N, offsets, E);
     W4_LAUNCH_CHECK();
     return W4_OK;
 }

@@ -705,7 +705,7 @@ int w4_s8_gemm_grouped(const int8_t *a, const float *a_scale, int a_rows, const 
     rc = w4::s8_gemm_grouped(a, a_rows, a_scale, w, w_scale, bias, offsets, rows, E, out,
                              c_dtype == W4_E4M3 ? W4_F32 : c_dtype, R, N, K, S(stream));
     if (rc || c_dtype != W4_E4M3) return rc;
-    return w4::rowscale_fp8(out, W4_F32, static_cast<uint8_t *>(c), row_scale, R, N, S(stream), offsets + E);
+    return w4::rowscale_fp8(out, W4_F32, static_cast<uint8_t *>(c), row_scale, R, N, S(stream), offsets, E);
 }
 
 size_t w4_moe_route_workspace_bytes(int T, int E) {

@@ -153,9 +153,9 @@ int nvfp4_prefill_q(const uint8_t *codes, const uint8_t *sfa, const float *a_glo
 size_t nvfp4_prefill_q_workspace(int M, int N, int K, bool scale_atoms_needed);
 // C = sum over splits of the fp32 partials [splits][mn] (mn % 4 == 0), in c_dtype (gptq_prefill.cu).
 int splitk_reduce(const float *partial, int splits, long mn, void *c, int c_dtype, cudaStream_t st);
-// limit (device, or null): rows from *limit on are left alone
+// offsets [E + 1] (device, or null): a grouped batch, whose rows of no expert are left alone
 int rowscale_fp8(const void *y, int y_dtype, uint8_t *q, float *row_scale, int M, int N,
-                 cudaStream_t st, const int *limit = nullptr);
+                 cudaStream_t st, const int *offsets = nullptr, int E = 0);
 // The same cast (bit for bit) from f32 y whose row maxima a decode GEMM folded into rowmax (fp32
 // bits, M <= 16); the last CTA of each row zeroes rowmax[row] again, counting on rowcnt[row].
 int rowscale_fp8_amax(const float *y, unsigned int *rowmax, unsigned int *rowcnt, uint8_t *q, float *row_scale,

@@ -507,7 +507,7 @@ def s8_gemm_grouped(a, a_scale, w, w_scale, offsets, rows=None, bias=None, out_d
     ``offsets``: i32 [E + 1] on the device (:func:`moe_route`), never read by the host.  ``rows``:
     i32 [R] on the device; row r of the batch is then row rows[r] of ``a`` [tokens, K] with its scale,
     so tokens are quantised once and never copied.  Without it ``a`` is the batch, [R, K].
-    Returns [R, N] (types as :func:`s8_gemm`); rows behind offsets[E] are not written.
+    Returns [R, N] (types as :func:`s8_gemm`); rows before offsets[0] and behind offsets[E] are not written.
     """
     if not torch.is_tensor(a) or a.dim() != 2 or not torch.is_tensor(w) or w.dim() != 3:
         raise ValueError("a must be [tokens, K] and w [E, N, K]")
