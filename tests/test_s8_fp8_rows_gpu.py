@@ -1,4 +1,5 @@
-"""The fp8 form of the grouped s8 GEMM casts the rows that the product wrote and no others."""
+"""The fp8 form of the grouped s8 GEMM casts the rows that the product wrote and no others; calls
+with no rows."""
 import numpy as np
 import pytest
 import torch
@@ -42,3 +43,20 @@ def test_fp8_rows_are_those_of_the_product(cuda, offsets, first, end, gather):
         q_ref, s_ref = O.rowscale_fp8(np_(y[first:end]))
         assert np.array_equal(np_(q.view(torch.uint8))[first:end], q_ref)
         assert np.array_equal(np_(s)[first:end], s_ref)
+
+
+def test_no_rows_are_gathered_from_some_tokens(cuda):
+    a, sa, w, sw = _setup()
+    off = torch.zeros(5, dtype=torch.int32, device=cuda)
+    none = torch.empty(0, dtype=torch.int32, device=cuda)
+    assert ops.s8_gemm_grouped(a, sa, w, sw, off, none).shape == (0, 130)
+    q, s = ops.s8_gemm_grouped(a, sa, w, sw, off, none, out_dtype=torch.float8_e4m3fn)
+    assert q.shape == (0, 130) and s.shape == (0,)
+
+
+def test_a_layer_without_tokens(cuda):
+    _, _, w, sw = _setup(4, 1, 256, 128)
+    wo, so = w.transpose(1, 2).contiguous()[:, :, :128].contiguous(), torch.ones(4, 128, device=cuda)
+    lay = ops.S8Experts(w, sw, wo, so, top_k=2)
+    assert lay(torch.empty(0, 128, device=cuda), torch.empty(0, 4, device=cuda)).shape == (0, 128)
+    assert ops.S8Linear(w[0], sw[0])(torch.empty(0, 128, device=cuda)).shape == (0, 256)

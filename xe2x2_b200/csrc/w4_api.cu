@@ -694,8 +694,9 @@ int w4_s8_gemm_grouped(const int8_t *a, const float *a_scale, int a_rows, const 
     if (rc) return rc;
     W4_REQUIRE(E >= 1, W4_ERR_INVALID, "E=%d", E);
     W4_REQUIRE(E <= w4::kMaxMoeExperts, W4_ERR_UNSUPPORTED, "E=%d exceeds %d experts", E, w4::kMaxMoeExperts);
-    W4_REQUIRE(a_rows >= 0 && (rows || a_rows == R), W4_ERR_INVALID, "a_rows=%d must be R=%d without rows", a_rows, R);
-    if (R == 0) return W4_OK;
+    W4_REQUIRE(a_rows >= 0, W4_ERR_INVALID, "a_rows=%d", a_rows);
+    if (R == 0) return W4_OK;  // an empty batch, whatever there is to gather from
+    W4_REQUIRE(rows || a_rows == R, W4_ERR_INVALID, "a_rows=%d must be R=%d without rows", a_rows, R);
     W4_REQUIRE(a_rows >= 1, W4_ERR_INVALID, "a has no rows to gather from");
     W4_REQUIRE(offsets && aligned(offsets, 4) && aligned(rows, 4), W4_ERR_INVALID,
                "offsets are required, offsets and rows 4-byte aligned");
