@@ -396,10 +396,14 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, const Token<EPL> &k, 
             }
             if (__any_sync(0xffffffffu, tie)) {
                 // The last one chosen ties with the one behind it, which says nothing of those behind that: each
-                // is compared with the last one here, and `from` for all that were not ranked.
+                // is compared with the last one here, and the largest of those that were not ranked.
                 const int le = __shfl_sync(0xffffffffu, c->e, a.k - 1);
                 const float x = from_ordered(__shfl_sync(0xffffffffu, mine, a.k - 1)), bx = a.bias[le];
-                near |= !done || x - from_ordered(from) <= close_to(a.softmax, 1.f, x);
+                uint32_t rest = 0;
+#pragma unroll
+                for (int i = 0; i < EPL; ++i) rest = max(rest, key[i] < from ? key[i] : 0u);
+                rest = warp_max(rest);
+                near |= !done || (rest != 0 && x - from_ordered(rest) <= close_to(a.softmax, 1.f, x));
                 if (done && lane > a.k && lane < n) {
                     const uint2 o = pick->out[lane];
                     const float y = from_ordered(o.x), by = a.bias[o.y];
