@@ -416,7 +416,9 @@ enum w4_moe_group_score {
  *     W4_GROUP_TOP2 of p + bias; only the topk_group best groups' experts can be chosen.
  *   - ids i32 [T, top_k], best first; equal scores go to the lower index.  Scores are compared
  *     in 64 bits (without a bias and group sums: as logits).
- *   - weights f32 [T, top_k] = scaling * p, divided by their sum with renorm (0 if that is 0).
+ *   - weights f32 [T, top_k] = scaling * p, divided by their sum with renorm (0 if that is 0); within
+ *     1e-6 (relative) of the formula, with softmax 1.2e-7 times the logit's distance from the largest
+ *     one more, and without renorm another 2.4e-6.
  * An expert whose logit is -inf (or whose bias is -inf or NaN) is never chosen.  A token that has
  * fewer than top_k experts to choose from gets id -1 and weight 0 in the slots left over, so a row
  * of -inf (padding) goes nowhere.  A NaN logit counts as -inf for the choice, and every weight of

@@ -21,7 +21,7 @@ namespace moe {
 // tell apart: the choice would depend on how exp was rounded.  So a token is first chosen for in 32
 // bits, with one rank more than asked for, and where two neighbours (or the last group kept and the
 // next) are closer than the 32-bit errors, it is chosen for again in 64 (under 1 % of the tokens; all
-// in 64 bits took 61 us for 8192 x 256, top 8 of 4 in 8 groups, where this takes 20).
+// in 64 bits took 61 us for 8192 x 256, top 8 of 4 in 8 groups, where this takes 21).
 //
 // The order by expert is a counting sort without atomics whose order matters: a token takes an
 // expert at most once, so a bit mask over a chunk's tokens for each expert gives counts (popc) and
@@ -498,8 +498,9 @@ __device__ __forceinline__ void route_token(const RouteArgs &a, int t, const flo
     if (!choose<EPL, float, uint32_t>(a, k, reinterpret_cast<float *>(base), lpg, pick, lane, &c))
         choose<EPL, double, uint64_t>(a, k, base, lpg, pick, lane, &c);
 
-    // Weights in 32 bits (the functions of the library, 1 ulp) unless a score is so small that it, or the
-    // sum, would be lost.
+    // Weights in 32 bits (expf and the quotient within an ulp) unless a score is so small that it, or the
+    // sum, would be lost.  A softmax that is not renormalised divides by the sum that choose() took, of
+    // base-2 exponentials of the hardware: within 2.4e-6 of itself (see close_to).
     const float l = c.e >= 0 ? fminf(logit_of(a, t, c.e), FLT_MAX) : 0.f;
     const float f = a.softmax ? expf(l - k.top) : __fdiv_rn(1.f, 1.f + expf(-l));
     float w = c.e >= 0 ? f : 0.f;
@@ -679,7 +680,7 @@ __global__ void __launch_bounds__(KT) place_kernel(const RouteArgs a) {
 
 // Threads and tokens of a CTA.  Up to 32 tokens one CTA does everything.  Up to 16 an SM: 16 warps, a token
 // each (148 tokens: 8.4 us, with 32 warps 11.6).  More: one CTA of 32 warps an SM (8192 tokens: 25 us where
-// two of 16 warps took 28, since every CTA of the second kernel reads all counts; 20 us since); at most 1024
+// two of 16 warps took 28, since every CTA of the second kernel reads all counts; 21 us since); at most 1024
 // tokens (the masks are E * chunk / 8 bytes of shared memory).
 struct Shape {
     int threads, chunk;
